@@ -35,6 +35,32 @@ SIGNATURES = {
     "fms_plain_backward_split": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _P, ctypes.c_size_t, _P],
 }
 
+
+
+class SsmArgs(ctypes.Structure):
+    """``fms_ssm_args`` of the header."""
+    _fields_ = [("batch", _I64), ("channels", _I64), ("groups", _I64), ("states", _I64), ("T", _I64), ("dtype", _I),
+                ("delta_softplus", _I), ("tokens", _P), ("delta", _P), ("z", _P), ("B", _P), ("C", _P),
+                ("tokens_stride", _I64 * 2), ("delta_stride", _I64 * 2), ("z_stride", _I64 * 2), ("B_stride", _I64 * 3),
+                ("C_stride", _I64 * 3), ("A", _P), ("D", _P), ("delta_bias", _P), ("h0", _P), ("lengths", _P)]
+
+
+class ConvArgs(ctypes.Structure):
+    """``fms_conv_args`` of the header."""
+    _fields_ = [("batch", _I64), ("channels", _I64), ("taps", _I64), ("T", _I64), ("dtype", _I), ("silu", _I),
+                ("tokens", _P), ("tokens_stride", _I64 * 2), ("weight", _P), ("bias", _P), ("x0", _P), ("lengths", _P)]
+
+
+_SSM, _CONV, _SIZE = ctypes.POINTER(SsmArgs), ctypes.POINTER(ConvArgs), ctypes.c_size_t
+SIGNATURES.update({
+    "fms_ssm_forward": [_SSM, _P, _P, _P, _P],
+    "fms_ssm_backward": [_SSM, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SIZE, _P],
+    "fms_ssm_step": [_SSM, _P, _I64, _P, _P, _P],
+    "fms_conv_forward": [_CONV, _P, _P, _P],
+    "fms_conv_backward": [_CONV, _P, _P, _P, _P, _P, _P, _P, _SIZE, _P],
+    "fms_conv_step": [_CONV, _P, _I64, _P, _P, _P],
+})
+
 _lib = None
 
 
@@ -70,6 +96,10 @@ def lib() -> ctypes.CDLL:
         L.fms_plain_split_workspace_bytes.argtypes = [_I64, _I64, _I]
         L.fms_fm_backward_workspace_bytes.restype = ctypes.c_size_t
         L.fms_fm_backward_workspace_bytes.argtypes = [_I64, _I64, _I64, _I64, _I]
+        for name, args in (("fms_ssm_checkpoint_bytes", _SSM), ("fms_ssm_backward_workspace_bytes", _SSM),
+                           ("fms_conv_backward_workspace_bytes", _CONV)):
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = _SIZE, [args]
         _lib = L
     return _lib
 

@@ -12,6 +12,10 @@
 
 #define FMS_EXPORT extern "C" __attribute__((visibility("default")))
 
+namespace fms {
+int record_cuda_error(cudaError_t e);  // for the other translation units of the C ABI
+}
+
 namespace {
 
 thread_local int g_last_cuda_error = 0;
@@ -348,6 +352,8 @@ int launch_combine(const float *P, const float *S, const float *carry0, float *c
     }
 
 }  // namespace
+
+int fms::record_cuda_error(cudaError_t e) { return record(e); }
 
 FMS_EXPORT int fms_version(void) { return 200; }
 

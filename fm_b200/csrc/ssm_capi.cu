@@ -1,0 +1,461 @@
+// C ABI of the selective state-space scan and its causal filter (see include/fm_scan_b200.h): argument
+// checks, launch shapes, launches.  No allocation, no synchronisation, no torch.
+#include "fm_scan_b200.h"
+
+#include <algorithm>
+
+#include "conv_kernels.cuh"
+#include "ssm_kernels.cuh"
+
+#define FMS_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace fms {
+int record_cuda_error(cudaError_t e);  // fm_scan_capi.cu: this thread's fms_last_cuda_error
+}
+
+namespace {
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr size_t kMaxSmem = 227 * 1024;  // of a CTA on sm_100
+
+inline int check_launch() { return fms::record_cuda_error(cudaGetLastError()); }
+inline bool dtype_ok(int d) { return d == FMS_F32 || d == FMS_F16 || d == FMS_BF16; }
+inline int64_t elem_size(int d) { return d == FMS_F32 ? 4 : 2; }
+inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// a * b * c * ... with every product below 2^59, so that byte offsets fit int64
+bool product_ok(std::initializer_list<int64_t> v) {
+    int64_t p = 1;
+    for (int64_t k : v) {
+        if (k < 0) return false;
+        if (k && p > (int64_t{1} << 59) / k) return false;
+        p *= k ? k : 1;
+    }
+    return true;
+}
+
+// every row of a tensor with these element strides starts on a 16-byte boundary
+bool rows16(const void *p, const int64_t *stride, int n, int64_t es) {
+    if (!aligned_to(p, 16)) return false;
+    for (int i = 0; i < n; ++i)
+        if (stride[i] * es % 16) return false;
+    return true;
+}
+
+int ssm_check(const fms_ssm_args *a) {
+    if (!a) return FMS_ERR_NULL_POINTER;
+    if (!dtype_ok(a->dtype)) return FMS_ERR_BAD_DTYPE;
+    if (a->batch < 0 || a->channels < 0 || a->T < 0 || a->groups < 1 || a->states < 1) return FMS_ERR_BAD_SHAPE;
+    if (a->channels % a->groups) return FMS_ERR_BAD_SHAPE;
+    if (a->states > FMS_SSM_MAX_STATES || a->T > 0x7fffffff - 4096) return FMS_ERR_TOO_LARGE;
+    if (!product_ok({a->batch, a->channels, std::max<int64_t>(a->T, a->states)}) ||
+        !product_ok({a->batch, a->groups, a->states, a->T}) ||
+        !product_ok({a->batch, a->channels, a->T / fms::kSsmTile + 1, a->states}))
+        return FMS_ERR_BAD_SHAPE;
+    return FMS_OK;
+}
+
+inline bool ssm_empty(const fms_ssm_args *a) { return a->batch == 0 || a->channels == 0; }
+
+int ssm_pointers(const fms_ssm_args *a, bool big) {
+    const size_t es = elem_size(a->dtype);
+    if (!a->A || (big && (!a->tokens || !a->delta || !a->B || !a->C))) return FMS_ERR_NULL_POINTER;
+    for (const void *p : {a->tokens, a->delta, a->z, a->B, a->C})
+        if (!aligned_to(p, es)) return FMS_ERR_MISALIGNED;
+    for (const float *p : {a->A, a->D, a->delta_bias, a->h0})
+        if (!aligned_to(p, 4)) return FMS_ERR_MISALIGNED;
+    if (!aligned_to(a->lengths, 8)) return FMS_ERR_MISALIGNED;
+    return FMS_OK;
+}
+
+bool ssm_aligned(const fms_ssm_args *a) {
+    const int64_t es = elem_size(a->dtype);
+    return a->T * es % 16 == 0 && rows16(a->tokens, a->tokens_stride, 2, es) && rows16(a->delta, a->delta_stride, 2, es) &&
+           (!a->z || rows16(a->z, a->z_stride, 2, es)) && rows16(a->B, a->B_stride, 3, es) &&
+           rows16(a->C, a->C_stride, 3, es);
+}
+
+template <typename S>
+fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, int cw, int warps) {
+    fms::SsmProblem<S> p;
+    p.x = static_cast<const S *>(a->tokens), p.delta = static_cast<const S *>(a->delta), p.z = static_cast<const S *>(a->z);
+    p.B = static_cast<const S *>(a->B), p.C = static_cast<const S *>(a->C);
+    std::copy_n(a->tokens_stride, 2, p.xs);
+    std::copy_n(a->delta_stride, 2, p.ds);
+    std::copy_n(a->z_stride, 2, p.zs);
+    std::copy_n(a->B_stride, 3, p.Bs);
+    std::copy_n(a->C_stride, 3, p.Cs);
+    p.A = a->A, p.D = a->D, p.bias = a->delta_bias, p.h0 = a->h0, p.lengths = a->lengths;
+    p.batch = a->batch, p.channels = a->channels, p.groups = a->groups;
+    p.T = static_cast<int>(a->T), p.N = static_cast<int>(a->states);
+    p.NP = (p.N + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB;
+    p.per_group = static_cast<int>(a->channels / a->groups);
+    p.cw = cw;
+    p.chunks = (p.per_group + cw * warps - 1) / (cw * warps);
+    p.tiles = static_cast<int>((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
+    p.softplus = a->delta_softplus != 0;
+    return p;
+}
+
+// Channels of a warp.  More of them spread the loads of B and C over more work and, backward, shrink
+// the partial sums of their gradients; fewer give more warps.
+int ssm_fwd_cw(const fms_ssm_args *a) {
+    const int64_t warps = a->batch * a->channels;
+    return warps >= 8 * 4096 ? 8 : warps >= 4 * 4096 ? 4 : warps >= 2 * 4096 ? 2 : 1;
+}
+size_t ssm_bwd_smem(int cw, int NP) {
+    return sizeof(float) * fms::kSsmBwdWarps * (64 * 32 + fms::ssm_bwd_floats(cw, NP));
+}
+int ssm_bwd_cw(const fms_ssm_args *a) {
+    const int NP = static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
+    int cw = a->batch * a->channels < 64 * 148 ? 4 : 8;
+    while (ssm_bwd_smem(cw, NP) > kMaxSmem) cw /= 2;  // 256 states: 2 channels fit
+    return cw;
+}
+
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t bytes) {
+    return fms::record_cuda_error(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+}
+
+__global__ void fill_kernel(const float *__restrict__ src, float *__restrict__ dst, int64_t n) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i < n) dst[i] = src ? src[i] : 0.f;
+}
+int copy_or_zero(const float *src, float *dst, int64_t n, cudaStream_t st) {
+    if (!dst || n == 0) return FMS_OK;
+    if ((n + 255) / 256 > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    fill_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(src, dst, n);
+    return check_launch();
+}
+
+int sum_slices(const float *part, float *out, int64_t n, int64_t count, int64_t stride, cudaStream_t st) {
+    if (!out || n == 0) return FMS_OK;
+    if ((n + 127) / 128 > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    fms::sum_slices_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, st>>>(part, out, n, count, stride);
+    return check_launch();
+}
+
+template <typename S, bool ALIGNED>
+int launch_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *ck, cudaStream_t st) {
+    const auto p = ssm_problem<S>(a, ssm_fwd_cw(a), fms::kSsmFwdWarps);
+    const int64_t grid = p.batch * p.groups * p.chunks;
+    if (grid > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    const size_t smem = sizeof(float) * fms::kSsmFwdWarps * fms::ssm_fwd_floats(p.cw, p.NP);
+    if (int rc = allow_smem(fms::ssm_forward_kernel<S, ALIGNED>, smem)) return rc;
+    fms::ssm_forward_kernel<S, ALIGNED><<<static_cast<unsigned>(grid), fms::kSsmFwdWarps * 32, smem, st>>>(
+        p, static_cast<S *>(out), h_last, ck);
+    return check_launch();
+}
+
+struct SsmScratch {
+    size_t bc, a, d, total;
+};
+SsmScratch ssm_scratch(const fms_ssm_args *a) {
+    const int64_t cw = ssm_bwd_cw(a), per = a->channels / a->groups;
+    const int64_t chunks = (per + cw * fms::kSsmBwdWarps - 1) / (cw * fms::kSsmBwdWarps);
+    const int64_t Tpad = (a->T + fms::kSsmTile - 1) / fms::kSsmTile * fms::kSsmTile;
+    SsmScratch s;
+    s.bc = round256(sizeof(float) * a->batch * a->groups * chunks * 2 * a->states * Tpad);
+    s.a = round256(sizeof(float) * a->batch * a->channels * a->states);
+    s.d = round256(sizeof(float) * a->batch * a->channels * 2);
+    s.total = s.bc + s.a + s.d;
+    return s;
+}
+
+template <typename S, bool ALIGNED>
+int launch_ssm_backward(const fms_ssm_args *a, fms::SsmGrads<S> o, S *dB, S *dC, float *dA, float *dD, float *dbias,
+                        char *ws, cudaStream_t st) {
+    const auto p = ssm_problem<S>(a, ssm_bwd_cw(a), fms::kSsmBwdWarps);
+    const SsmScratch sc = ssm_scratch(a);
+    o.bc_part = reinterpret_cast<float *>(ws);
+    o.a_part = reinterpret_cast<float *>(ws + sc.bc);
+    o.d_part = reinterpret_cast<float *>(ws + sc.bc + sc.a);
+    const int64_t grid = p.batch * p.groups * p.chunks, rows = p.batch * p.groups * 2 * p.N;
+    if (grid > kMaxGrid || rows > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    const size_t smem = ssm_bwd_smem(p.cw, p.NP);
+    auto kernel = p.z ? fms::ssm_backward_kernel<S, ALIGNED, true> : fms::ssm_backward_kernel<S, ALIGNED, false>;
+    if (int rc = allow_smem(kernel, smem)) return rc;
+    kernel<<<static_cast<unsigned>(grid), fms::kSsmBwdWarps * 32, smem, st>>>(p, o);
+    if (int rc = check_launch()) return rc;
+    const int Tpad = p.tiles * fms::kSsmTile;
+    const dim3 g2(static_cast<unsigned>(rows), static_cast<unsigned>(std::min((p.T + 255) / 256, 65535)));
+    fms::ssm_bc_kernel<S><<<g2, 256, 0, st>>>(o.bc_part, dB, dC, p.groups, p.chunks, p.N, p.T, Tpad);
+    if (int rc = check_launch()) return rc;
+    if (int rc = sum_slices(o.a_part, dA, p.channels * p.N, p.batch, p.channels * p.N, st)) return rc;
+    if (int rc = sum_slices(o.d_part, dD, p.channels, p.batch, 2 * p.channels, st)) return rc;
+    return sum_slices(o.d_part + p.channels, dbias, p.channels, p.batch, 2 * p.channels, st);
+}
+
+template <typename S>
+int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
+    const auto p = ssm_problem<S>(a, 1, 1);
+    int L = 1;
+    while (L < 32 && 4 * L < p.N) L *= 2;
+    const int64_t blocks = (p.channels + 128 / L - 1) / (128 / L);
+    if (blocks > kMaxGrid || p.batch * blocks > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    const unsigned grid = static_cast<unsigned>(p.batch * blocks);
+    if (p.N % 4 == 0 && aligned_to(state, 16) && aligned_to(p.A, 16))
+        fms::ssm_step_kernel<S, true><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), L, static_cast<int>(blocks));
+    else
+        fms::ssm_step_kernel<S, false><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), L, static_cast<int>(blocks));
+    return check_launch();
+}
+
+// ------------------------------------------------------------------------------- filter ----
+
+int conv_check(const fms_conv_args *a) {
+    if (!a) return FMS_ERR_NULL_POINTER;
+    if (!dtype_ok(a->dtype)) return FMS_ERR_BAD_DTYPE;
+    if (a->batch < 0 || a->channels < 0 || a->T < 0 || a->taps < 2 || a->taps > 8) return FMS_ERR_BAD_SHAPE;
+    if (a->T > 0x7fffffff - 4096) return FMS_ERR_TOO_LARGE;
+    if (!product_ok({a->batch, a->channels, std::max<int64_t>(a->T, 16)})) return FMS_ERR_BAD_SHAPE;
+    return FMS_OK;
+}
+int conv_pointers(const fms_conv_args *a) {
+    if (!a->weight || (a->T && !a->tokens)) return FMS_ERR_NULL_POINTER;
+    const size_t es = elem_size(a->dtype);
+    if (!aligned_to(a->tokens, es) || !aligned_to(a->x0, es) || !aligned_to(a->weight, 4) || !aligned_to(a->bias, 4) ||
+        !aligned_to(a->lengths, 8))
+        return FMS_ERR_MISALIGNED;
+    return FMS_OK;
+}
+bool conv_aligned(const fms_conv_args *a) {
+    const int64_t es = elem_size(a->dtype);
+    return a->T * es % 16 == 0 && rows16(a->tokens, a->tokens_stride, 2, es);
+}
+
+int conv_lanes(int64_t T) {
+    int lpr = 1;
+    while (lpr < 32 && lpr * 8 < T) lpr *= 2;
+    return lpr;
+}
+int64_t conv_chunks(int64_t T) {
+    const int64_t span = static_cast<int64_t>(conv_lanes(T)) * 8 * fms::kConvUnroll;
+    return std::max<int64_t>(1, (T + span - 1) / span);
+}
+
+template <typename S>
+fms::ConvProblem<S> conv_problem(const fms_conv_args *a) {
+    fms::ConvProblem<S> p;
+    p.x = static_cast<const S *>(a->tokens);
+    std::copy_n(a->tokens_stride, 2, p.xs);
+    p.weight = a->weight, p.bias = a->bias, p.x0 = static_cast<const S *>(a->x0), p.lengths = a->lengths;
+    p.batch = a->batch, p.channels = a->channels, p.chunks = conv_chunks(a->T);
+    p.T = static_cast<int>(a->T), p.lpr = conv_lanes(a->T), p.silu = a->silu != 0;
+    return p;
+}
+template <typename S>
+int64_t conv_grid(const fms::ConvProblem<S> &p) {
+    const int64_t per = 32 / p.lpr, units = (p.batch * p.channels + per - 1) / per * p.chunks;
+    return (units + fms::kConvWarps - 1) / fms::kConvWarps;
+}
+
+template <typename S, int K, bool ALIGNED>
+int launch_conv_forward(const fms_conv_args *a, void *out, void *x_last, cudaStream_t st) {
+    const auto p = conv_problem<S>(a);
+    if (conv_grid(p) > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    fms::conv_forward_kernel<S, K, ALIGNED><<<static_cast<unsigned>(conv_grid(p)), fms::kConvWarps * 32, 0, st>>>(
+        p, static_cast<S *>(out), static_cast<S *>(x_last));
+    return check_launch();
+}
+
+template <typename S, int K, bool ALIGNED>
+int launch_conv_backward(const fms_conv_args *a, const void *dout, const void *dlast, void *dx, float *dw, float *db,
+                         void *dx0, float *part, cudaStream_t st) {
+    const auto p = conv_problem<S>(a);
+    if (conv_grid(p) > kMaxGrid || (p.channels + 3) / 4 > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    fms::conv_backward_kernel<S, K, ALIGNED><<<static_cast<unsigned>(conv_grid(p)), fms::kConvWarps * 32, 0, st>>>(
+        p, static_cast<const S *>(dout), static_cast<const S *>(dlast), static_cast<S *>(dx), static_cast<S *>(dx0), part);
+    if (int rc = check_launch()) return rc;
+    fms::conv_weight_kernel<K><<<static_cast<unsigned>((p.channels + 3) / 4), 128, 0, st>>>(part, dw, db, p.batch,
+                                                                                         p.channels, p.chunks);
+    return check_launch();
+}
+
+template <typename S, int K>
+int launch_conv_step(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
+    const auto p = conv_problem<S>(a);
+    const int64_t blocks = (p.channels + 127) / 128;
+    if (blocks > kMaxGrid || p.batch * blocks > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    fms::conv_step_kernel<S, K><<<static_cast<unsigned>(p.batch * blocks), 128, 0, st>>>(
+        p, static_cast<S *>(state), pool, slots, static_cast<S *>(out), static_cast<int>(blocks));
+    return check_launch();
+}
+
+}  // namespace
+
+#define FMS_BY_TYPE(dtype, CALL)                                         \
+    switch (dtype) {                                                     \
+        case FMS_F32: { using S = float; return CALL; }                  \
+        case FMS_F16: { using S = __half; return CALL; }                 \
+        default: { using S = __nv_bfloat16; return CALL; }               \
+    }
+#define FMS_BY_TAPS(taps, CALL)                                          \
+    switch (taps) {                                                      \
+        case 2: { constexpr int K = 2; return CALL; }                    \
+        case 3: { constexpr int K = 3; return CALL; }                    \
+        case 4: { constexpr int K = 4; return CALL; }                    \
+        case 5: { constexpr int K = 5; return CALL; }                    \
+        case 6: { constexpr int K = 6; return CALL; }                    \
+        case 7: { constexpr int K = 7; return CALL; }                    \
+        default: { constexpr int K = 8; return CALL; }                   \
+    }
+
+namespace {
+template <typename S>
+int conv_forward_t(const fms_conv_args *a, void *out, void *x_last, cudaStream_t st) {
+    if (conv_aligned(a) && aligned_to(out, 16)) FMS_BY_TAPS(a->taps, (launch_conv_forward<S, K, true>(a, out, x_last, st)));
+    FMS_BY_TAPS(a->taps, (launch_conv_forward<S, K, false>(a, out, x_last, st)));
+}
+template <typename S>
+int conv_backward_t(const fms_conv_args *a, const void *dout, const void *dlast, void *dx, float *dw, float *db, void *dx0,
+                    float *part, cudaStream_t st) {
+    if (conv_aligned(a) && aligned_to(dout, 16) && aligned_to(dx, 16))
+        FMS_BY_TAPS(a->taps, (launch_conv_backward<S, K, true>(a, dout, dlast, dx, dw, db, dx0, part, st)));
+    FMS_BY_TAPS(a->taps, (launch_conv_backward<S, K, false>(a, dout, dlast, dx, dw, db, dx0, part, st)));
+}
+template <typename S>
+int conv_step_t(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
+    FMS_BY_TAPS(a->taps, (launch_conv_step<S, K>(a, state, pool, slots, out, st)));
+}
+template <typename S>
+int ssm_forward_t(const fms_ssm_args *a, void *out, float *h_last, float *ck, cudaStream_t st) {
+    return ssm_aligned(a) && aligned_to(out, 16) ? launch_ssm_forward<S, true>(a, out, h_last, ck, st)
+                                                 : launch_ssm_forward<S, false>(a, out, h_last, ck, st);
+}
+}  // namespace
+
+FMS_EXPORT size_t fms_ssm_checkpoint_bytes(const fms_ssm_args *a) {
+    if (ssm_check(a) != FMS_OK || ssm_empty(a)) return 0;
+    return sizeof(float) * a->batch * a->channels * a->states * ((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
+}
+
+FMS_EXPORT int fms_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *checkpoints, fms_stream_t stream) {
+    if (int rc = ssm_check(a)) return rc;
+    if (ssm_empty(a)) return FMS_OK;
+    if (int rc = ssm_pointers(a, a->T > 0)) return rc;
+    if (a->T > 0 && !out) return FMS_ERR_NULL_POINTER;
+    if (!aligned_to(out, elem_size(a->dtype)) || !aligned_to(h_last, 4) || !aligned_to(checkpoints, 4)) return FMS_ERR_MISALIGNED;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->T == 0) return copy_or_zero(a->h0, h_last, a->batch * a->channels * a->states, st);
+    FMS_BY_TYPE(a->dtype, (ssm_forward_t<S>(a, out, h_last, checkpoints, st)));
+}
+
+FMS_EXPORT size_t fms_ssm_backward_workspace_bytes(const fms_ssm_args *a) {
+    if (ssm_check(a) != FMS_OK || ssm_empty(a) || a->T == 0) return 0;
+    return ssm_scratch(a).total;
+}
+
+FMS_EXPORT int fms_ssm_backward(const fms_ssm_args *a, const float *checkpoints, const void *grad_out,
+                                const float *grad_last, void *grad_tokens, void *grad_delta, void *grad_z, void *grad_B,
+                                void *grad_C, float *grad_A, float *grad_D, float *grad_delta_bias, float *grad_h0,
+                                void *workspace, size_t workspace_bytes, fms_stream_t stream) {
+    if (int rc = ssm_check(a)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t states = a->batch * a->channels * a->states;
+    if (a->channels == 0) return FMS_OK;
+    if (!grad_A) return FMS_ERR_NULL_POINTER;
+    for (const float *p : {checkpoints, grad_last, static_cast<const float *>(grad_A), static_cast<const float *>(grad_D),
+                           static_cast<const float *>(grad_delta_bias), static_cast<const float *>(grad_h0)})
+        if (!aligned_to(p, 4)) return FMS_ERR_MISALIGNED;
+    if (a->batch == 0 || a->T == 0) {  // nothing was read but h0, which went to the last state
+        if (int rc = copy_or_zero(nullptr, grad_A, a->channels * a->states, st)) return rc;
+        if (int rc = copy_or_zero(nullptr, grad_D, a->channels, st)) return rc;
+        if (int rc = copy_or_zero(nullptr, grad_delta_bias, a->channels, st)) return rc;
+        return copy_or_zero(grad_last, grad_h0, states, st);
+    }
+    if (int rc = ssm_pointers(a, true)) return rc;
+    if (!checkpoints || !grad_out || !grad_tokens || !grad_delta || !grad_B || !grad_C || (a->z && !grad_z))
+        return FMS_ERR_NULL_POINTER;
+    const int64_t es = elem_size(a->dtype);
+    bool all16 = ssm_aligned(a);
+    for (const void *p : {grad_out, static_cast<const void *>(grad_tokens), static_cast<const void *>(grad_delta),
+                          static_cast<const void *>(grad_z), static_cast<const void *>(grad_B), static_cast<const void *>(grad_C)}) {
+        if (!aligned_to(p, es)) return FMS_ERR_MISALIGNED;
+        all16 = all16 && aligned_to(p, 16);
+    }
+    if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < fms_ssm_backward_workspace_bytes(a))
+        return FMS_ERR_WORKSPACE;
+    auto go = [&](auto tag) -> int {
+        using S = decltype(tag);
+        fms::SsmGrads<S> o{};
+        o.checkpoints = checkpoints;
+        o.grad_out = static_cast<const S *>(grad_out);
+        o.grad_last = grad_last;
+        o.dx = static_cast<S *>(grad_tokens), o.ddelta = static_cast<S *>(grad_delta), o.dz = static_cast<S *>(grad_z);
+        o.dh0 = grad_h0;
+        auto *dB = static_cast<S *>(grad_B), *dC = static_cast<S *>(grad_C);
+        char *ws = static_cast<char *>(workspace);
+        return all16 ? launch_ssm_backward<S, true>(a, o, dB, dC, grad_A, grad_D, grad_delta_bias, ws, st)
+                     : launch_ssm_backward<S, false>(a, o, dB, dC, grad_A, grad_D, grad_delta_bias, ws, st);
+    };
+    FMS_BY_TYPE(a->dtype, go(S{}));
+}
+
+FMS_EXPORT int fms_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int64_t *slots, void *out,
+                            fms_stream_t stream) {
+    if (int rc = ssm_check(a)) return rc;
+    if (a->T != 1 || pool < 0 || (!slots && pool < a->batch)) return FMS_ERR_BAD_SHAPE;
+    if (!product_ok({pool, a->channels, a->states})) return FMS_ERR_BAD_SHAPE;
+    if (ssm_empty(a)) return FMS_OK;
+    if (int rc = ssm_pointers(a, true)) return rc;
+    if (!out || (pool && !state)) return FMS_ERR_NULL_POINTER;
+    if (!aligned_to(state, 4) || !aligned_to(slots, 8) || !aligned_to(out, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    FMS_BY_TYPE(a->dtype, (launch_ssm_step<S>(a, state, pool, slots, out, st)));
+}
+
+FMS_EXPORT int fms_conv_forward(const fms_conv_args *a, void *out, void *x_last, fms_stream_t stream) {
+    if (int rc = conv_check(a)) return rc;
+    if (a->batch == 0 || a->channels == 0) return FMS_OK;
+    if (int rc = conv_pointers(a)) return rc;
+    if (a->T && !out) return FMS_ERR_NULL_POINTER;
+    if (!aligned_to(out, elem_size(a->dtype)) || !aligned_to(x_last, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
+    if (a->T == 0 && !x_last) return FMS_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    FMS_BY_TYPE(a->dtype, (conv_forward_t<S>(a, out, x_last, st)));
+}
+
+FMS_EXPORT size_t fms_conv_backward_workspace_bytes(const fms_conv_args *a) {
+    if (conv_check(a) != FMS_OK || a->batch == 0 || a->channels == 0) return 0;
+    return round256(sizeof(float) * a->batch * a->channels * conv_chunks(a->T) * (a->taps + 1));
+}
+
+FMS_EXPORT int fms_conv_backward(const fms_conv_args *a, const void *grad_out, const void *grad_last, void *grad_tokens,
+                                 float *grad_weight, float *grad_bias, void *grad_x0, void *workspace,
+                                 size_t workspace_bytes, fms_stream_t stream) {
+    if (int rc = conv_check(a)) return rc;
+    if (a->channels == 0) return FMS_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!grad_weight) return FMS_ERR_NULL_POINTER;
+    if (!aligned_to(grad_weight, 4) || !aligned_to(grad_bias, 4)) return FMS_ERR_MISALIGNED;
+    if (a->batch == 0) {
+        if (int rc = copy_or_zero(nullptr, grad_weight, a->channels * a->taps, st)) return rc;
+        return copy_or_zero(nullptr, grad_bias, a->channels, st);
+    }
+    if (int rc = conv_pointers(a)) return rc;
+    if (a->T && (!grad_out || !grad_tokens)) return FMS_ERR_NULL_POINTER;
+    for (const void *p : {grad_out, grad_last, static_cast<const void *>(grad_tokens), static_cast<const void *>(grad_x0)})
+        if (!aligned_to(p, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
+    if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < fms_conv_backward_workspace_bytes(a))
+        return FMS_ERR_WORKSPACE;
+    FMS_BY_TYPE(a->dtype, (conv_backward_t<S>(a, grad_out, grad_last, grad_tokens, grad_weight, grad_bias, grad_x0,
+                                              static_cast<float *>(workspace), st)));
+}
+
+FMS_EXPORT int fms_conv_step(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out,
+                             fms_stream_t stream) {
+    if (int rc = conv_check(a)) return rc;
+    if (a->T != 1 || pool < 0 || (!slots && pool < a->batch)) return FMS_ERR_BAD_SHAPE;
+    if (!product_ok({pool, a->channels, 8})) return FMS_ERR_BAD_SHAPE;
+    if (a->batch == 0 || a->channels == 0) return FMS_OK;
+    if (int rc = conv_pointers(a)) return rc;
+    if (!out || (pool && !state)) return FMS_ERR_NULL_POINTER;
+    if (!aligned_to(state, elem_size(a->dtype)) || !aligned_to(slots, 8) || !aligned_to(out, elem_size(a->dtype)))
+        return FMS_ERR_MISALIGNED;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    FMS_BY_TYPE(a->dtype, (conv_step_t<S>(a, state, pool, slots, out, st)));
+}

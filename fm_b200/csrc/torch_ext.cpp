@@ -401,6 +401,234 @@ void fm_scan_backward(const at::Tensor &gates, const at::Tensor &outGrad,
                         c10::nullopt, c10::nullopt);
 }
 
+// ------------------------------------------------------------ selective state-space layer ----
+// Outputs are allocated here, on the tensors' device and the current stream's pool.
+
+using OptTensor = c10::optional<at::Tensor>;
+
+static bool given(const OptTensor &t) { return t.has_value() && t->defined(); }
+
+static void want_rows(const at::Tensor &t, const at::Tensor &like, at::IntArrayRef shape, const char *name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == like.device(), name, " must be on the device of tokens");
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the dtype of tokens");
+    TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+    TORCH_CHECK(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, name, " must have a contiguous last axis");
+}
+
+static const float *want_f32(const OptTensor &t, const at::Tensor &like, at::IntArrayRef shape, const char *name) {
+    if (!given(t)) return nullptr;
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), name, " must be a CUDA tensor on the device of tokens");
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous(), name, " must be contiguous float32");
+    TORCH_CHECK(t->sizes() == shape, name, " must have shape ", shape, ", got ", t->sizes());
+    return t->data_ptr<float>();
+}
+
+static const int64_t *want_index(const OptTensor &t, const at::Tensor &like, int64_t n, const char *name) {
+    if (!given(t)) return nullptr;
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), name, " must be a CUDA tensor on the device of tokens");
+    TORCH_CHECK(t->scalar_type() == at::kLong && t->is_contiguous() && t->dim() == 1 && t->size(0) == n, name,
+                " must be a contiguous integer tensor with one element per sequence (", n, ")");
+    return t->data_ptr<int64_t>();
+}
+
+static void strides_of(const at::Tensor &t, int n, int64_t *to) {
+    for (int i = 0; i < n; ++i) to[i] = t.stride(i);
+}
+
+// Fills args from the tensors of a scan (time: last axis) or, with step, of one token (no time axis).
+static fms_ssm_args ssm_args(const at::Tensor &x, const at::Tensor &delta, const at::Tensor &A, const at::Tensor &B,
+                             const at::Tensor &C, const OptTensor &D, const OptTensor &z, const OptTensor &bias,
+                             const OptTensor &h0, const OptTensor &lengths, bool softplus, bool step) {
+    const char *shape = step ? "(B, D)" : "(B, D, T)";
+    const int axes = step ? 2 : 3;
+    TORCH_CHECK(x.is_cuda(), "tokens must be a CUDA tensor (there is no CPU path)");
+    TORCH_CHECK(x.dim() == axes, "tokens must be ", shape);
+    TORCH_CHECK(A.dim() == 2, "A must be (D, N)");
+    TORCH_CHECK(B.dim() == axes || B.dim() == axes + 1, "B must be ", step ? "(B, N) or (B, G, N)" : "(B, N, T) or (B, G, N, T)");
+    fms_ssm_args a{};
+    a.batch = x.size(0), a.channels = x.size(1), a.T = step ? 1 : x.size(2);
+    a.states = A.size(1);
+    const bool grouped = B.dim() == axes + 1;
+    a.groups = grouped ? B.size(1) : 1;
+    TORCH_CHECK(a.groups >= 1 && a.channels % a.groups == 0, "the groups of B must divide the channels");
+    TORCH_CHECK(a.states >= 1 && a.states <= FMS_SSM_MAX_STATES, "A must have 1 to ", FMS_SSM_MAX_STATES, " states");
+    a.dtype = dtype_tag(x);
+    a.delta_softplus = softplus;
+    std::vector<int64_t> rows = {a.batch, a.channels}, bc = {a.batch};
+    if (grouped) bc.push_back(a.groups);
+    bc.push_back(a.states);
+    if (!step) rows.push_back(a.T), bc.push_back(a.T);
+    want_rows(x, x, rows, "tokens");
+    want_rows(delta, x, rows, "delta");
+    want_rows(B, x, bc, "B");
+    want_rows(C, x, bc, "C");
+    a.tokens = x.data_ptr(), a.delta = delta.data_ptr(), a.B = B.data_ptr(), a.C = C.data_ptr();
+    strides_of(x, 2, a.tokens_stride);
+    strides_of(delta, 2, a.delta_stride);
+    if (given(z)) {
+        want_rows(*z, x, rows, "z");
+        a.z = z->data_ptr();
+        strides_of(*z, 2, a.z_stride);
+    }
+    auto bc_strides = [&](const at::Tensor &t, int64_t *to) {
+        to[0] = t.stride(0);
+        to[1] = grouped ? t.stride(1) : 0;
+        to[2] = t.stride(grouped ? 2 : 1);
+    };
+    bc_strides(B, a.B_stride);
+    bc_strides(C, a.C_stride);
+    a.A = want_f32(A, x, {a.channels, a.states}, "A");
+    a.D = want_f32(D, x, {a.channels}, "D");
+    a.delta_bias = want_f32(bias, x, {a.channels}, "delta_bias");
+    a.h0 = want_f32(h0, x, {a.batch, a.channels, a.states}, "initial_state");
+    a.lengths = want_index(lengths, x, a.batch, "lengths");
+    return a;
+}
+
+static std::tuple<at::Tensor, OptTensor, OptTensor> ssm_forward(
+    const at::Tensor &x, const at::Tensor &delta, const at::Tensor &A, const at::Tensor &B, const at::Tensor &C,
+    const OptTensor &D, const OptTensor &z, const OptTensor &bias, const OptTensor &h0, const OptTensor &lengths,
+    bool softplus, bool want_last, bool want_checkpoints) {
+    const fms_ssm_args a = ssm_args(x, delta, A, B, C, D, z, bias, h0, lengths, softplus, false);
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = at::empty(x.sizes(), x.options());
+    OptTensor last, ck;
+    if (want_last) last = at::empty({a.batch, a.channels, a.states}, A.options());
+    if (want_checkpoints) ck = at::empty({static_cast<int64_t>(fms_ssm_checkpoint_bytes(&a) / 4)}, A.options());
+    check_status(fms_ssm_forward(&a, out.data_ptr(), want_last ? last->data_ptr<float>() : nullptr,
+                                 want_checkpoints ? ck->data_ptr<float>() : nullptr,
+                                 at::cuda::getCurrentCUDAStream().stream()),
+                 "ssm_scan");
+    return {out, last, ck};
+}
+
+// grads of tokens, delta, A, B, C, D, z, delta_bias, initial_state (None where the input is)
+static std::vector<OptTensor> ssm_backward(
+    const at::Tensor &x, const at::Tensor &delta, const at::Tensor &A, const at::Tensor &B, const at::Tensor &C,
+    const OptTensor &D, const OptTensor &z, const OptTensor &bias, const OptTensor &h0, const OptTensor &lengths,
+    bool softplus, const OptTensor &checkpoints, const at::Tensor &grad_out, const OptTensor &grad_last) {
+    const fms_ssm_args a = ssm_args(x, delta, A, B, C, D, z, bias, h0, lengths, softplus, false);
+    const c10::cuda::CUDAGuard guard(x.device());
+    want_rows(grad_out, x, x.sizes(), "grad_out");
+    TORCH_CHECK(grad_out.is_contiguous(), "grad_out must be contiguous");
+    TORCH_CHECK(given(checkpoints), "the forward kept no states for a backward");
+    const float *gl = want_f32(grad_last, x, {a.batch, a.channels, a.states}, "grad_last");
+    at::Tensor dx = at::empty(x.sizes(), x.options()), dd = at::empty(x.sizes(), x.options());
+    at::Tensor dA = at::empty(A.sizes(), A.options()), dB = at::empty(B.sizes(), x.options()), dC = at::empty(C.sizes(), x.options());
+    OptTensor dD, dz, db, dh;
+    if (given(D)) dD = at::empty(D->sizes(), D->options());
+    if (given(z)) dz = at::empty(x.sizes(), x.options());
+    if (given(bias)) db = at::empty(bias->sizes(), bias->options());
+    if (given(h0)) dh = at::empty(h0->sizes(), h0->options());
+    const size_t scratch = fms_ssm_backward_workspace_bytes(&a);
+    at::Tensor ws = at::empty({static_cast<int64_t>(std::max<size_t>(scratch, 16))}, x.options().dtype(at::kByte));
+    auto f = [](const OptTensor &t) { return given(t) ? t->data_ptr<float>() : nullptr; };
+    check_status(fms_ssm_backward(&a, f(checkpoints), grad_out.data_ptr(), gl, dx.data_ptr(), dd.data_ptr(),
+                                  given(z) ? dz->data_ptr() : nullptr, dB.data_ptr(), dC.data_ptr(), dA.data_ptr<float>(),
+                                  f(dD), f(db), f(dh), ws.data_ptr(), scratch, at::cuda::getCurrentCUDAStream().stream()),
+                 "ssm_scan backward");
+    return {dx, dd, dA, dB, dC, dD, dz, db, dh};
+}
+
+static at::Tensor ssm_step(const at::Tensor &x, const at::Tensor &delta, const at::Tensor &state, const at::Tensor &A,
+                           const at::Tensor &B, const at::Tensor &C, const OptTensor &D, const OptTensor &z,
+                           const OptTensor &bias, bool softplus, const OptTensor &slots) {
+    const fms_ssm_args a = ssm_args(x, delta, A, B, C, D, z, bias, c10::nullopt, c10::nullopt, softplus, true);
+    TORCH_CHECK(state.dim() == 3, "state must be (pool, D, N)");
+    const float *st = want_f32(state, x, {state.size(0), a.channels, a.states}, "state");
+    const int64_t *at_ = want_index(slots, x, a.batch, "slots");
+    TORCH_CHECK(at_ || !(a.batch > state.size(0)), "state must hold one state per row when slots is omitted");
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = at::empty(x.sizes(), x.options());
+    check_status(fms_ssm_step(&a, const_cast<float *>(st), state.size(0), at_, out.data_ptr(),
+                              at::cuda::getCurrentCUDAStream().stream()),
+                 "ssm_step");
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
+static fms_conv_args conv_args(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias, const OptTensor &x0,
+                               const OptTensor &lengths, bool silu, bool step) {
+    TORCH_CHECK(x.is_cuda(), "tokens must be a CUDA tensor (there is no CPU path)");
+    TORCH_CHECK(x.dim() == (step ? 2 : 3), "tokens must be ", step ? "(B, D)" : "(B, D, T)");
+    TORCH_CHECK(weight.dim() == 2 && weight.size(1) >= 2 && weight.size(1) <= 8, "weight must be (D, K) with 2 to 8 taps");
+    fms_conv_args a{};
+    a.batch = x.size(0), a.channels = x.size(1), a.T = step ? 1 : x.size(2), a.taps = weight.size(1);
+    a.dtype = dtype_tag(x);
+    a.silu = silu;
+    want_rows(x, x, x.sizes(), "tokens");
+    a.tokens = x.data_ptr();
+    strides_of(x, 2, a.tokens_stride);
+    a.weight = want_f32(weight, x, {a.channels, a.taps}, "weight");
+    a.bias = want_f32(bias, x, {a.channels}, "bias");
+    if (given(x0)) {
+        want_rows(*x0, x, {a.batch, a.channels, a.taps - 1}, "initial_state");
+        TORCH_CHECK(x0->is_contiguous(), "initial_state must be contiguous");
+        a.x0 = x0->data_ptr();
+    }
+    a.lengths = want_index(lengths, x, a.batch, "lengths");
+    return a;
+}
+
+static std::tuple<at::Tensor, OptTensor> short_conv_forward(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias,
+                                                            const OptTensor &x0, const OptTensor &lengths, bool silu,
+                                                            bool want_last) {
+    const fms_conv_args a = conv_args(x, weight, bias, x0, lengths, silu, false);
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = at::empty(x.sizes(), x.options());
+    OptTensor last;
+    if (want_last) last = at::empty({a.batch, a.channels, a.taps - 1}, x.options());
+    check_status(fms_conv_forward(&a, out.data_ptr(), want_last ? last->data_ptr() : nullptr,
+                                  at::cuda::getCurrentCUDAStream().stream()),
+                 "short_conv");
+    return {out, last};
+}
+
+// grads of tokens, weight, bias, initial_state (None where the input is)
+static std::vector<OptTensor> short_conv_backward(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias,
+                                                  const OptTensor &x0, const OptTensor &lengths, bool silu,
+                                                  const at::Tensor &grad_out, const OptTensor &grad_last) {
+    const fms_conv_args a = conv_args(x, weight, bias, x0, lengths, silu, false);
+    const c10::cuda::CUDAGuard guard(x.device());
+    want_rows(grad_out, x, x.sizes(), "grad_out");
+    TORCH_CHECK(grad_out.is_contiguous(), "grad_out must be contiguous");
+    const void *gl = nullptr;
+    if (given(grad_last)) {
+        want_rows(*grad_last, x, {a.batch, a.channels, a.taps - 1}, "grad_last");
+        TORCH_CHECK(grad_last->is_contiguous(), "grad_last must be contiguous");
+        gl = grad_last->data_ptr();
+    }
+    at::Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty(weight.sizes(), weight.options());
+    OptTensor db, d0;
+    if (given(bias)) db = at::empty(bias->sizes(), bias->options());
+    if (given(x0)) d0 = at::empty(x0->sizes(), x0->options());
+    const size_t scratch = fms_conv_backward_workspace_bytes(&a);
+    at::Tensor ws = at::empty({static_cast<int64_t>(std::max<size_t>(scratch, 16))}, x.options().dtype(at::kByte));
+    check_status(fms_conv_backward(&a, grad_out.data_ptr(), gl, dx.data_ptr(), dw.data_ptr<float>(),
+                                   given(bias) ? db->data_ptr<float>() : nullptr, given(x0) ? d0->data_ptr() : nullptr,
+                                   ws.data_ptr(), scratch, at::cuda::getCurrentCUDAStream().stream()),
+                 "short_conv backward");
+    return {dx, dw, db, d0};
+}
+
+static at::Tensor short_conv_step(const at::Tensor &x, const at::Tensor &state, const at::Tensor &weight, const OptTensor &bias,
+                                  bool silu, const OptTensor &slots) {
+    const fms_conv_args a = conv_args(x, weight, bias, c10::nullopt, c10::nullopt, silu, true);
+    TORCH_CHECK(state.dim() == 3, "state must be (pool, D, K-1)");
+    want_rows(state, x, {state.size(0), a.channels, a.taps - 1}, "state");
+    TORCH_CHECK(state.is_contiguous(), "state must be contiguous");
+    const int64_t *at_ = want_index(slots, x, a.batch, "slots");
+    TORCH_CHECK(at_ || !(a.batch > state.size(0)), "state must hold one state per row when slots is omitted");
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = at::empty(x.sizes(), x.options());
+    check_status(fms_conv_step(&a, state.data_ptr(), state.size(0), at_, out.data_ptr(),
+                               at::cuda::getCurrentCUDAStream().stream()),
+                 "short_conv_step");
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "fm_scan for B200: torch shim over the C ABI libfm_scan_b200.so";
     m.def("fm_scan_forward", &fm_scan_forward, "scan forward (writes and returns out)");
@@ -412,5 +640,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fm_memory_forward_train", &fm_memory_forward_train, "layer forward: output + normalised states");
     m.def("fm_memory_backward", &fm_memory_backward, "layer backward with the state gradient generated in-kernel");
     m.def("fm_memory_readout", &fm_memory_readout, "layer read-out without materialising the states");
+    m.def("ssm_forward", &ssm_forward, "state-space scan forward: out, last state, checkpoints");
+    m.def("ssm_backward", &ssm_backward, "state-space scan backward: gradients of every input");
+    m.def("ssm_step", &ssm_step, "state-space scan of one token, states advanced in place");
+    m.def("short_conv_forward", &short_conv_forward, "causal filter forward: out, last inputs");
+    m.def("short_conv_backward", &short_conv_backward, "causal filter backward: gradients of every input");
+    m.def("short_conv_step", &short_conv_step, "causal filter of one token, state shifted in place");
     m.def("abi_version", []() { return fms_version(); });
 }

@@ -399,6 +399,98 @@ int fms_tsplit_backward(const void *gates, const void *states, const void *grad_
                         void *const *peer_buffers, int world, int rank, uint32_t exchange, double max_wait_seconds,
                         fms_stream_t stream);
 
+/* ------------------------------------------- selective state-space layer: scan and filter ---- */
+
+/*
+ * A scan whose decay depends on the input and on N states per channel, and the short causal filter
+ * that stands in front of it, for whole sequences (forward and backward) and for single tokens.  The
+ * reference has one state per (memory, channel) and no such layer; the conventions are those of this
+ * library: (B, D, T) rows with time last, fp32 arithmetic and states, caller-owned scratch.
+ *
+ *   dt[b,d,t]   = delta[b,d,t] + delta_bias[d], through log(1 + exp(.)) when delta_softplus != 0
+ *   h[b,d,n,t]  = exp(dt * A[d,n]) * h[b,d,n,t-1] + dt * B[b,g,n,t] * x[b,d,t]        g = d / (D/G)
+ *   y[b,d,t]    = sum_n C[b,g,n,t] * h[b,d,n,t] + D[d] * x[b,d,t]
+ *   out[b,d,t]  = y * z * sigmoid(z)  where z is given, else y
+ *
+ * Every large tensor has time as its last axis with stride 1; the other strides are given in elements
+ * and need not be those of a contiguous tensor (0 included, for inputs).  Tensors the library writes
+ * are contiguous.  lengths[b] (nullable, int64 on the device, clamped to [0, T]) ends sequence b
+ * early: positions from there on are never read into a result, their outputs and gradients are zero,
+ * and the last state is the state at lengths[b].
+ */
+typedef struct fms_ssm_args {
+    int64_t batch, channels, groups, states, T;  /* B, D, G (divides D), N (1 ... FMS_SSM_MAX_STATES), T >= 0 */
+    int dtype;                                   /* of tokens, delta, z, B, C and the outputs           */
+    int delta_softplus;
+    const void *tokens, *delta, *z;              /* (B, D, T); z nullable                               */
+    const void *B, *C;                           /* (B, G, N, T)                                        */
+    int64_t tokens_stride[2], delta_stride[2], z_stride[2]; /* batch, channel                           */
+    int64_t B_stride[3], C_stride[3];            /* batch, group, state                                 */
+    const float *A;                              /* (D, N) fp32, contiguous, finite                     */
+    const float *D, *delta_bias;                 /* (D) fp32, nullable                                  */
+    const float *h0;                             /* (B, D, N) fp32, nullable = zeros                    */
+    const int64_t *lengths;                      /* (B), nullable = T everywhere                        */
+} fms_ssm_args;
+#define FMS_SSM_MAX_STATES 256
+
+/*
+ * Forward.  out (B, D, T); h_last (B, D, N) fp32, nullable; checkpoints: nullable, fp32, of
+ * fms_ssm_checkpoint_bytes(), receives the states the backward starts its blocks of positions from.
+ */
+size_t fms_ssm_checkpoint_bytes(const fms_ssm_args *args);
+int fms_ssm_forward(const fms_ssm_args *args, void *out, float *h_last, float *checkpoints, fms_stream_t stream);
+
+/*
+ * Backward of the above from grad_out (B, D, T, contiguous) and grad_last (B, D, N) fp32, nullable.
+ * checkpoints are the forward's.  Outputs: grad_tokens, grad_delta, grad_z (iff z) of the storage type,
+ * contiguous (B, D, T); grad_B, grad_C of the storage type, contiguous (B, G, N, T); grad_A (D, N) fp32;
+ * grad_D, grad_delta_bias (D) fp32 and grad_h0 (B, D, N) fp32, nullable.  Sums over channels, time and
+ * batch run in a fixed order: equal calls give equal bits.
+ */
+size_t fms_ssm_backward_workspace_bytes(const fms_ssm_args *args);
+int fms_ssm_backward(const fms_ssm_args *args, const float *checkpoints, const void *grad_out,
+                     const float *grad_last, void *grad_tokens, void *grad_delta, void *grad_z, void *grad_B,
+                     void *grad_C, float *grad_A, float *grad_D, float *grad_delta_bias, float *grad_h0,
+                     void *workspace, size_t workspace_bytes, fms_stream_t stream);
+
+/*
+ * One token: args->T is 1, tokens, delta, z are (B, D) and B, C are (B, G, N) with the LAST axis of
+ * stride 1 (tokens_stride[0] etc. are the batch strides, B_stride[0..1] batch and group; the other
+ * stride fields, h0 and lengths are not read).  state: (pool, D, N) fp32, contiguous, advanced in place.
+ * slots: (B) int64 on the device, nullable = row b uses state b (pool >= B).  A row whose slot lies
+ * outside [0, pool), or was already named by an earlier row, is padding: its output is zero and no
+ * state changes for it.
+ */
+int fms_ssm_step(const fms_ssm_args *args, float *state, int64_t pool, const int64_t *slots, void *out,
+                 fms_stream_t stream);
+
+/*
+ * The filter: out[b,d,t] = act(bias[d] + sum_k weight[d,k] * x[b,d,t-K+1+k]), act the identity or
+ * v * sigmoid(v).  Positions before 0 come from x0 (B, D, K-1), contiguous, nullable = zeros; x_last
+ * (B, D, K-1), nullable, receives the last K-1 inputs of every sequence (of x0 followed by the tokens).
+ */
+typedef struct fms_conv_args {
+    int64_t batch, channels, taps, T;     /* taps K: 2 ... 8                                            */
+    int dtype;                            /* of tokens, x0, x_last and the outputs                      */
+    int silu;                             /* 0: act is the identity                                     */
+    const void *tokens;                   /* (B, D, T), time stride 1                                   */
+    int64_t tokens_stride[2];             /* batch, channel                                             */
+    const float *weight, *bias;           /* (D, K) and (D) fp32; bias nullable                         */
+    const void *x0;
+    const int64_t *lengths;               /* (B), nullable                                              */
+} fms_conv_args;
+
+int fms_conv_forward(const fms_conv_args *args, void *out, void *x_last, fms_stream_t stream);
+/* grad_x0 (B, D, K-1) of the storage type, grad_last likewise: nullable.  grad_bias nullable. */
+size_t fms_conv_backward_workspace_bytes(const fms_conv_args *args);
+int fms_conv_backward(const fms_conv_args *args, const void *grad_out, const void *grad_last, void *grad_tokens,
+                      float *grad_weight, float *grad_bias, void *grad_x0, void *workspace, size_t workspace_bytes,
+                      fms_stream_t stream);
+/* One token: args->T is 1, tokens (B, D) with tokens_stride[0] the batch stride and channels of stride 1;
+ * state (pool, D, K-1) of the storage type, shifted by one token in place; slots as in fms_ssm_step. */
+int fms_conv_step(const fms_conv_args *args, void *state, int64_t pool, const int64_t *slots, void *out,
+                  fms_stream_t stream);
+
 /* ------------------------------------------------------- host-buffer pipeline (one GPU) ---- */
 
 /*
