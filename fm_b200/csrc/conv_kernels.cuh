@@ -19,6 +19,44 @@ namespace fms {
 constexpr int kConvUnroll = 4;  // tiles of a unit
 constexpr int kConvWarps = 4;
 
+// Positions [t, t + 8) of a row as floats; positions from `lim` on are zero and not read.  ALIGNED: the
+// row starts on a 16-byte boundary and t is a multiple of 8.
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ void load8(const S *__restrict__ row, int t, int lim, float (&f)[8]) {
+    if (ALIGNED && t + 8 <= lim) {
+        if constexpr (sizeof(S) == 4) {
+            const float4 p = __ldg(reinterpret_cast<const float4 *>(row + t));
+            const float4 q = __ldg(reinterpret_cast<const float4 *>(row + t) + 1);
+            f[0] = p.x, f[1] = p.y, f[2] = p.z, f[3] = p.w;
+            f[4] = q.x, f[5] = q.y, f[6] = q.z, f[7] = q.w;
+        } else {
+            const uint4 p = __ldg(reinterpret_cast<const uint4 *>(row + t));
+            Store<S>::unpack(p, f);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = t + i < lim ? Store<S>::to_float(row[t + i]) : 0.f;
+    }
+}
+
+// Stores positions [t, t + 8) of a row, those below `T` only.
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ void store8(S *__restrict__ row, int t, int T, const float (&f)[8]) {
+    if (ALIGNED && t + 8 <= T) {
+        if constexpr (sizeof(S) == 4) {
+            float4 *o = reinterpret_cast<float4 *>(row + t);
+            o[0] = make_float4(f[0], f[1], f[2], f[3]);
+            o[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *reinterpret_cast<uint4 *>(row + t) = Store<S>::pack(f);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (t + i < T) row[t + i] = from_float<S>(f[i]);
+    }
+}
+
 template <typename S>
 struct ConvProblem {
     const S *x;

@@ -3,6 +3,7 @@
 #include "fm_scan_b200.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "conv_kernels.cuh"
 #include "ssm_kernels.cuh"
@@ -98,21 +99,43 @@ fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, int cw, int warps) {
     return p;
 }
 
-// Channels of a warp.  More of them spread the loads of B and C over more work and, backward, shrink
-// the partial sums of their gradients; fewer give more warps.
-int ssm_fwd_cw(const fms_ssm_args *a) {
-    const int64_t warps = a->batch * a->channels;
-    return warps >= 8 * 4096 ? 8 : warps >= 4 * 4096 ? 4 : warps >= 2 * 4096 ? 2 : 1;
+inline int padded_states(const fms_ssm_args *a) {
+    return static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
 }
-size_t ssm_bwd_smem(int cw, int NP) {
-    return sizeof(float) * fms::kSsmBwdWarps * (64 * 32 + fms::ssm_bwd_floats(cw, NP));
+
+// shared memory of a CTA: as the kernels lay it out
+size_t ssm_fwd_smem(const fms_ssm_args *a, int cw) {
+    return a->dtype == FMS_F32
+               ? fms::ssm_bc_bytes<float>() + fms::kSsmFwdWarps * fms::ssm_fwd_warp_bytes<float>(cw, padded_states(a))
+               : fms::ssm_bc_bytes<__half>() + fms::kSsmFwdWarps * fms::ssm_fwd_warp_bytes<__half>(cw, padded_states(a));
 }
-int ssm_bwd_cw(const fms_ssm_args *a) {
-    const int NP = static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
-    int cw = a->batch * a->channels < 64 * 148 ? 4 : 8;
-    while (ssm_bwd_smem(cw, NP) > kMaxSmem) cw /= 2;  // 256 states: 2 channels fit
-    return cw;
+size_t ssm_bwd_smem(const fms_ssm_args *a, int cw) {
+    const size_t red = sizeof(float) * fms::kSsmBwdWarps * 64 * 32;
+    return red + (a->dtype == FMS_F32
+                      ? fms::ssm_bc_bytes<float>() + fms::kSsmBwdWarps * fms::ssm_bwd_warp_bytes<float>(cw, padded_states(a))
+                      : fms::ssm_bc_bytes<__half>() + fms::kSsmBwdWarps * fms::ssm_bwd_warp_bytes<__half>(cw, padded_states(a)));
 }
+
+// Channels of a warp.  More of them spread a tile's B, C and barriers over more work (and, backward,
+// shrink the partial sums of their gradients); fewer give more warps.  The time is taken as the number
+// of waves times the channels of a warp plus the share of a channel that a tile costs on its own.
+int best_cw(const fms_ssm_args *a, int warps, int most, int per_sm, double own, size_t (*smem)(const fms_ssm_args *, int)) {
+    const int64_t per = a->channels / a->groups;
+    int best = 1;
+    double least = 0;
+    for (int cw = 1; cw <= most; ++cw) {
+        const size_t bytes = smem(a, cw);
+        if (bytes > kMaxSmem) break;
+        const int64_t ctas = a->batch * a->groups * ((per + cw * warps - 1) / (cw * warps));
+        const int64_t room = 148 * std::min<int64_t>(per_sm, static_cast<int64_t>((kMaxSmem + 1024) / (bytes + 1024)));
+        const double t = static_cast<double>((ctas + room - 1) / room) * (cw + own);
+        if (cw == 1 || t < least) best = cw, least = t;
+    }
+    return best;
+}
+int env_int(const char *name, int dflt) { const char *s = std::getenv(name); return s ? std::atoi(s) : dflt; }
+int ssm_fwd_cw(const fms_ssm_args *a) { if (int v = env_int("X_FCW", 0)) return v; return best_cw(a, fms::kSsmFwdWarps, 8, 3, 1.5, ssm_fwd_smem); }
+int ssm_bwd_cw(const fms_ssm_args *a) { if (int v = env_int("X_BCW", 0)) return v; return best_cw(a, fms::kSsmBwdWarps, 8, 1, 1.5, ssm_bwd_smem); }
 
 template <typename Kernel>
 int allow_smem(Kernel kernel, size_t bytes) {
@@ -143,7 +166,7 @@ int launch_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *c
     const auto p = ssm_problem<S>(a, ssm_fwd_cw(a), fms::kSsmFwdWarps);
     const int64_t grid = p.batch * p.groups * p.chunks;
     if (grid > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    const size_t smem = sizeof(float) * fms::kSsmFwdWarps * fms::ssm_fwd_floats(p.cw, p.NP);
+    const size_t smem = ssm_fwd_smem(a, p.cw);
     if (int rc = allow_smem(fms::ssm_forward_kernel<S, ALIGNED>, smem)) return rc;
     fms::ssm_forward_kernel<S, ALIGNED><<<static_cast<unsigned>(grid), fms::kSsmFwdWarps * 32, smem, st>>>(
         p, static_cast<S *>(out), h_last, ck);
@@ -175,7 +198,7 @@ int launch_ssm_backward(const fms_ssm_args *a, fms::SsmGrads<S> o, S *dB, S *dC,
     o.d_part = reinterpret_cast<float *>(ws + sc.bc + sc.a);
     const int64_t grid = p.batch * p.groups * p.chunks, rows = p.batch * p.groups * 2 * p.N;
     if (grid > kMaxGrid || rows > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    const size_t smem = ssm_bwd_smem(p.cw, p.NP);
+    const size_t smem = ssm_bwd_smem(a, p.cw);
     auto kernel = p.z ? fms::ssm_backward_kernel<S, ALIGNED, true> : fms::ssm_backward_kernel<S, ALIGNED, false>;
     if (int rc = allow_smem(kernel, smem)) return rc;
     kernel<<<static_cast<unsigned>(grid), fms::kSsmBwdWarps * 32, smem, st>>>(p, o);

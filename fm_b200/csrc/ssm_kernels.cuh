@@ -7,14 +7,22 @@
 // grid of 8 time lanes x 4 state lanes; a lane holds 8 consecutive positions of 4 states, so the 16
 // states of a block and the 64 positions of a tile are spread over the warp, and B and C of the tile
 // stay in registers while the warp goes through its channels.  Per channel and state a lane
-//   1. forms its 8 decays (one exponential each) and its aggregate (P, S): P = exp(A * sum dt) of its
-//      positions, S their state from a zero start,
+//   1. forms its 8 decays (one exponential each) and its aggregate (P, S): P the product of the decays,
+//      S the state of its positions from a zero start,
 //   2. takes part in a 3-step shuffle scan of the pairs over the 8 time lanes, seeded with the carry,
 //   3. runs its 8 positions again from the state that enters them, in registers.
 // Each decay is thus computed once and the sequence is parallel over positions, channels and states;
 // a thread per channel that walks time alone needs 64 x fewer positions in flight but fills the
 // machine only from some 40000 channels on, and its two-pass split along time computes every decay
-// twice.  The exponentials bound the forward: 16 per clock and SM.
+// twice.
+//
+// Rates that shape the code, measured per SM quarter: an exponential takes 8 cycles per warp, a
+// shuffle 4, a packed pair of fp32 multiply-adds 2 (one issue slot instead of two), a 16-byte
+// shared-memory load 16 whatever its lanes share.  Hence the exponentials bound the forward (8 cycles
+// per warp and 32 states), multiply-adds and issue slots the backward; work that is the same for all
+// states of a position (time step, gate) is done once per position, two positions a lane; multiply-adds
+// over positions are packed in pairs; and the tile's inputs come through shared memory, copied
+// asynchronously one tile ahead: B and C once for the CTA, the rows once per warp.
 #pragma once
 
 #include "scan_kernels.cuh"
@@ -46,6 +54,7 @@ struct SsmProblem {
     int softplus;
 };
 
+// ------------------------------------------------------------------------------ arithmetic ----
 __device__ __forceinline__ float ex2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -53,9 +62,47 @@ __device__ __forceinline__ float ex2(float v) {
 }
 __device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + ex2(-kLog2e * v)); }
 
-// log(1 + exp(v)); beyond 20 the two agree to fp32's last bit.  Once per position, not per state, so
-// the accurate library functions cost little; sigmoid_f is its derivative.
-__device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) in (0, 1].  log1p(e) = 2 artanh(r) with
+// r = e / (2 + e) <= 1/3, by its power series 2 (r + r^3/3 + r^5/5 + ...): the first term left out, at
+// r^17, is below 2^-26 of the sum, and small e keep their relative precision.  sigmoid_f is its derivative.
+__device__ __forceinline__ float softplus_f(float v) {
+    const float e = ex2(-kLog2e * fabsf(v));
+    const float r = __fdividef(e, 2.f + e), q = r * r;
+    float s = 1.f / 15.f;
+    s = fmaf(s, q, 1.f / 13.f);
+    s = fmaf(s, q, 1.f / 11.f);
+    s = fmaf(s, q, 1.f / 9.f);
+    s = fmaf(s, q, 1.f / 7.f);
+    s = fmaf(s, q, 1.f / 5.f);
+    s = fmaf(s, q, 1.f / 3.f);
+    s = fmaf(s * q, r, r);
+    return v != v ? v : fmaf(2.f, s, fmaxf(v, 0.f));
+}
+
+// two fp32 values in one 64-bit register pair; one instruction works on both
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pk(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float lo(f2 v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi(f2 v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 template <typename S>
 __device__ __forceinline__ S from_float(float f);
@@ -66,75 +113,138 @@ __device__ __forceinline__ __half from_float<__half>(float f) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float f) { return __float2bfloat16_rn(f); }
 
-// Positions [t, t + 8) of a row as floats; positions from `lim` on are zero and not read.  ALIGNED: the
-// row starts on a 16-byte boundary and t is a multiple of 8.
-template <typename S, bool ALIGNED>
-__device__ __forceinline__ void load8(const S *__restrict__ row, int t, int lim, float (&f)[8]) {
-    if (ALIGNED && t + 8 <= lim) {
-        if constexpr (sizeof(S) == 4) {
-            const float4 p = __ldg(reinterpret_cast<const float4 *>(row + t));
-            const float4 q = __ldg(reinterpret_cast<const float4 *>(row + t) + 1);
-            f[0] = p.x, f[1] = p.y, f[2] = p.z, f[3] = p.w;
-            f[4] = q.x, f[5] = q.y, f[6] = q.z, f[7] = q.w;
-        } else {
-            const uint4 p = __ldg(reinterpret_cast<const uint4 *>(row + t));
-            Store<S>::unpack(p, f);
+template <typename S>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+
+// --------------------------------------------------------------------- a row's tile, staged ----
+// 64 positions of a row lie in shared memory as they are in global memory: whole 16-byte granules,
+// from the one that holds the first position; rows that do not start on a 16-byte boundary need one
+// granule more.  What lies behind `lim` is filled with zeros and not read.
+template <typename S>
+__host__ __device__ constexpr int row_bytes() { return kSsmTile * static_cast<int>(sizeof(S)) + 16; }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Thread `i` of `n` copies its granules of `rows` rows; src(row) gives a row's first position (t = 0), or
+// null for a row of zeros.  `any`: some valid address, named by the copies that read nothing.
+template <typename S, bool ALIGNED, typename Src>
+__device__ __forceinline__ void stage_rows(unsigned char *to, int rows, int t0, int lim, int i, int n, const void *any,
+                                           Src src) {
+    constexpr int G = kSsmTile * static_cast<int>(sizeof(S)) / 16 + (ALIGNED ? 0 : 1);
+    const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    const int step_row = n / G, step_g = n - step_row * G;
+    int row = i / G, g = i - row * G;
+    while (row < rows) {
+        const S *first = src(row);
+        int left = 0;
+        const unsigned char *from = nullptr;
+        if (first) {
+            from = reinterpret_cast<const unsigned char *>(first + t0);
+            const unsigned char *end = reinterpret_cast<const unsigned char *>(first + lim);
+            if (!ALIGNED) from -= reinterpret_cast<uintptr_t>(from) & 15;
+            from += g * 16;
+            const int64_t d = end - from;
+            left = d < 0 ? 0 : d > 16 ? 16 : static_cast<int>(d);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = t + i < lim ? Store<S>::to_float(row[t + i]) : 0.f;
+        copy16(base + row * row_bytes<S>() + g * 16, left ? static_cast<const void *>(from) : any, left);
+        row += step_row;
+        g += step_g;
+        if (g >= G) {
+            g -= G;
+            ++row;
+        }
     }
 }
 
-// Stores positions [t, t + 8) of a row, those below `T` only.
+// Element offset of a staged row's first position inside its first granule.
 template <typename S, bool ALIGNED>
-__device__ __forceinline__ void store8(S *__restrict__ row, int t, int T, const float (&f)[8]) {
-    if (ALIGNED && t + 8 <= T) {
-        if constexpr (sizeof(S) == 4) {
-            float4 *o = reinterpret_cast<float4 *>(row + t);
-            o[0] = make_float4(f[0], f[1], f[2], f[3]);
-            o[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ int row_shift(const S *first) {
+    return ALIGNED ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / sizeof(S));
+}
+
+// positions 2l, 2l + 1 of a staged row
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ float2 row_pair(const unsigned char *row, int shift, int l) {
+    const S *p = reinterpret_cast<const S *>(row) + shift + 2 * l;
+    if constexpr (ALIGNED) {
+        if constexpr (sizeof(S) == 4) return *reinterpret_cast<const float2 *>(p);
+        else return unpack2<S>(*reinterpret_cast<const uint32_t *>(p));
+    } else {
+        return make_float2(Store<S>::to_float(p[0]), Store<S>::to_float(p[1]));
+    }
+}
+
+// positions 8s ... 8s + 7 of a staged row, as 4 packed pairs
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ void row_eight(const unsigned char *row, int shift, int s, f2 (&o)[4]) {
+    const S *p = reinterpret_cast<const S *>(row) + shift + 8 * s;
+    if constexpr (sizeof(S) == 4) {
+        if constexpr (ALIGNED) {
+            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+            o[0] = pk(a.x, a.y), o[1] = pk(a.z, a.w), o[2] = pk(b.x, b.y), o[3] = pk(b.z, b.w);
         } else {
-            *reinterpret_cast<uint4 *>(row + t) = Store<S>::pack(f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = pk(Store<S>::to_float(p[2 * k]), Store<S>::to_float(p[2 * k + 1]));
         }
     } else {
+        uint32_t w[4];
+        if constexpr (ALIGNED) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(p);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {  // five words around the eight halfwords, shifted by one halfword where they start odd
+            const bool odd = shift & 1;
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(p - (odd ? 1 : 0));
+            uint32_t v = q[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (t + i < T) row[t + i] = from_float<S>(f[i]);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t next = (odd || k < 3) ? q[k + 1] : 0u;
+                w[k] = odd ? __funnelshift_r(v, next, 16) : v;
+                v = next;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<S>(w[k]);
+            o[k] = pk(f.x, f.y);
+        }
     }
 }
 
 // A tile's 64 floats in shared memory: time lane s keeps positions 8s ... 8s+3 at [4s] and the other
-// four at [32 + 4s], so that 8 time lanes read or write 128 contiguous bytes.
-__device__ __forceinline__ void tile_get(const float *base, int s, float (&f)[8]) {
+// four at [32 + 4s], so that 8 time lanes read or write 128 contiguous bytes.  pair_at: positions 2l, 2l + 1.
+__device__ __forceinline__ int pair_at(int l) { return (l & 2) * 16 + (l >> 2) * 4 + (l & 1) * 2; }
+__device__ __forceinline__ void tile_get(const float *base, int s, f2 (&f)[4]) {
     const float4 p = *reinterpret_cast<const float4 *>(base + 4 * s);
     const float4 q = *reinterpret_cast<const float4 *>(base + 32 + 4 * s);
-    f[0] = p.x, f[1] = p.y, f[2] = p.z, f[3] = p.w;
-    f[4] = q.x, f[5] = q.y, f[6] = q.z, f[7] = q.w;
-}
-__device__ __forceinline__ void tile_put(float *base, int s, const float (&f)[8]) {
-    *reinterpret_cast<float4 *>(base + 4 * s) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4 *>(base + 32 + 4 * s) = make_float4(f[4], f[5], f[6], f[7]);
+    f[0] = pk(p.x, p.y), f[1] = pk(p.z, p.w), f[2] = pk(q.x, q.y), f[3] = pk(q.z, q.w);
 }
 
 // Sum of v over the 4 state lanes, spread so that each of them keeps two positions: state lane q gets
 // positions 4 * (q & 1) + 2 * (q >> 1) and the next.  `fresh`: the pair replaces what the tile holds.
-__device__ __forceinline__ void tile_sum(float *base, int s, int q, const float (&v)[8], bool fresh) {
-    const bool hi = q & 1, hi2 = q >> 1;
+__device__ __forceinline__ void tile_sum(float *base, int s, int q, const f2 (&v)[4], bool fresh) {
+    const bool up = q & 1, up2 = q >> 1;
     float r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float keep = hi ? v[i + 4] : v[i], give = hi ? v[i] : v[i + 4];
-        r[i] = keep + __shfl_xor_sync(kFullMask, give, 8);
+        const float a = i & 1 ? hi(v[i >> 1]) : lo(v[i >> 1]), b = i & 1 ? hi(v[2 + (i >> 1)]) : lo(v[2 + (i >> 1)]);
+        r[i] = (up ? b : a) + __shfl_xor_sync(kFullMask, up ? a : b, 8);
     }
     float2 o;
-    {
-        const float k0 = hi2 ? r[2] : r[0], g0 = hi2 ? r[0] : r[2];
-        const float k1 = hi2 ? r[3] : r[1], g1 = hi2 ? r[1] : r[3];
-        o.x = k0 + __shfl_xor_sync(kFullMask, g0, 16);
-        o.y = k1 + __shfl_xor_sync(kFullMask, g1, 16);
-    }
-    float2 *at = reinterpret_cast<float2 *>(base + (hi ? 32 : 0) + 4 * s + (hi2 ? 2 : 0));
+    o.x = (up2 ? r[2] : r[0]) + __shfl_xor_sync(kFullMask, up2 ? r[0] : r[2], 16);
+    o.y = (up2 ? r[3] : r[1]) + __shfl_xor_sync(kFullMask, up2 ? r[1] : r[3], 16);
+    float2 *at = reinterpret_cast<float2 *>(base + (up ? 32 : 0) + 4 * s + (up2 ? 2 : 0));
     if (!fresh) {
         const float2 old = *at;
         o.x += old.x;
@@ -143,30 +253,28 @@ __device__ __forceinline__ void tile_sum(float *base, int s, int q, const float 
     *at = o;
 }
 
-// Inclusive scan of (P, S) over the 8 time lanes; lane 0's S is already the true state.
-__device__ __forceinline__ float scan_up(float P, float S, int s) {
+// Inclusive scan of (P, S) over the 8 time lanes, towards higher or lower lanes; the first lane's S is
+// already the true state.  Returns the state that enters the lane; `S` becomes the one that leaves it.
+template <bool UP>
+__device__ __forceinline__ float lane_scan(float P, float &S, float carry, int s) {
+    const int r = UP ? s : 7 - s;
+    if (r == 0) S = fmaf(P, carry, S);
 #pragma unroll
     for (int k = 1; k < 8; k *= 2) {
-        const float Sp = __shfl_up_sync(kFullMask, S, k, 8);
-        const float Pp = k < 4 ? __shfl_up_sync(kFullMask, P, k, 8) : 0.f;
-        if (s >= k) {
+        const float Sp = UP ? __shfl_up_sync(kFullMask, S, k, 8) : __shfl_down_sync(kFullMask, S, k, 8);
+        float Pp = 0.f;
+        if (k < 4) Pp = UP ? __shfl_up_sync(kFullMask, P, k, 8) : __shfl_down_sync(kFullMask, P, k, 8);
+        if (r >= k) {
             S = fmaf(P, Sp, S);
             P *= Pp;
         }
     }
-    return S;
+    const float in = UP ? __shfl_up_sync(kFullMask, S, 1, 8) : __shfl_down_sync(kFullMask, S, 1, 8);
+    return r == 0 ? carry : in;
 }
-__device__ __forceinline__ float scan_down(float P, float S, int s) {
-#pragma unroll
-    for (int k = 1; k < 8; k *= 2) {
-        const float Sp = __shfl_down_sync(kFullMask, S, k, 8);
-        const float Pp = k < 4 ? __shfl_down_sync(kFullMask, P, k, 8) : 0.f;
-        if (s + k < 8) {
-            S = fmaf(P, Sp, S);
-            P *= Pp;
-        }
-    }
-    return S;
+__device__ __forceinline__ float product8(const f2 (&a)[4]) {
+    const f2 m = mul2(mul2(a[0], a[1]), mul2(a[2], a[3]));
+    return lo(m) * hi(m);
 }
 
 // Which channels a warp has: [c0, c0 + nc) of group g of sequence b; nc may be <= 0.
@@ -177,10 +285,9 @@ struct SsmPlace {
 template <typename S>
 __device__ __forceinline__ SsmPlace ssm_place(const SsmProblem<S> &p, int warps) {
     SsmPlace w;
-    const int per = p.chunks;
     int64_t k = blockIdx.x;
-    w.chunk = static_cast<int>(k % per);
-    k /= per;
+    w.chunk = static_cast<int>(k % p.chunks);
+    k /= p.chunks;
     w.g = static_cast<int>(k % p.groups);
     w.b = k / p.groups;
     const int c0 = (w.chunk * warps + static_cast<int>(threadIdx.x >> 5)) * p.cw;
@@ -195,130 +302,186 @@ __device__ __forceinline__ int ssm_length(const SsmProblem<S> &p, int64_t b) {
     return static_cast<int>(n < 0 ? 0 : n > p.T ? p.T : n);
 }
 
-// dt of 8 raw values; positions from lim on get 0, which makes them the identity step.
-template <typename S>
-__device__ __forceinline__ void time_steps(const SsmProblem<S> &p, float bias, int t, int lim, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float r = v[i] + bias;
-        v[i] = t + i < lim ? (p.softplus ? softplus_f(r) : r) : 0.f;
+// Time step of a raw value; a position behind the sequence gets 0, which makes it the identity step.
+__device__ __forceinline__ float time_step(float raw, float bias, int softplus, bool live) {
+    const float r = raw + bias;
+    return live ? (softplus ? softplus_f(r) : r) : 0.f;
+}
+
+// Positions t, t + 1 of an output row, those below T only.
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ void store_pair(S *__restrict__ row, int t, int T, float a, float b) {
+    if (ALIGNED && t + 2 <= T) {
+        if constexpr (sizeof(S) == 4) {
+            *reinterpret_cast<float2 *>(row + t) = make_float2(a, b);
+        } else {
+            union {
+                S h[2];
+                uint32_t w;
+            } v;
+            v.h[0] = from_float<S>(a);
+            v.h[1] = from_float<S>(b);
+            *reinterpret_cast<uint32_t *>(row + t) = v.w;
+        }
+    } else {
+        if (t < T) row[t] = from_float<S>(a);
+        if (t + 1 < T) row[t + 1] = from_float<S>(b);
     }
 }
 
-// floats of shared memory a warp needs
-inline __host__ __device__ int ssm_fwd_floats(int cw, int NP) { return cw * (3 * kSsmTile + 2 * NP); }
-inline __host__ __device__ int ssm_bwd_floats(int cw, int NP) { return cw * (6 * kSsmTile + 4 * NP + 4); }
+// bytes of shared memory: forward per CTA and warp; backward likewise
+template <typename S>
+inline __host__ __device__ size_t ssm_bc_bytes() { return 2 * 2 * kSsmNB * row_bytes<S>(); }
+template <typename S>
+inline __host__ __device__ size_t ssm_fwd_warp_bytes(int cw, int NP) {
+    return cw * (2 * 3 * row_bytes<S>() + sizeof(float) * (3 * kSsmTile + 2 * NP));
+}
+template <typename S>
+inline __host__ __device__ size_t ssm_bwd_warp_bytes(int cw, int NP) {
+    return cw * (2 * 4 * row_bytes<S>() + sizeof(float) * (6 * kSsmTile + 4 * NP + 4));
+}
 
 template <typename S, bool ALIGNED>
 __global__ void __launch_bounds__(kSsmFwdWarps * 32)
 ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict__ h_last,
                    float *__restrict__ checkpoints) {
-    extern __shared__ __align__(16) float ssm_smem[];
+    extern __shared__ __align__(16) unsigned char ssm_smem[];
+    constexpr int RB = row_bytes<S>();
     const int lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3;
     const SsmPlace w = ssm_place(p, kSsmFwdWarps);
-    if (w.nc <= 0) return;
-    float *dt_ = ssm_smem + (threadIdx.x >> 5) * ssm_fwd_floats(p.cw, p.NP);
+    unsigned char *raw = ssm_smem + ssm_bc_bytes<S>() + (threadIdx.x >> 5) * ssm_fwd_warp_bytes<S>(p.cw, p.NP);
+    float *dt_ = reinterpret_cast<float *>(raw + 2 * 3 * p.cw * RB);
     float *u_ = dt_ + p.cw * kSsmTile, *y_ = u_ + p.cw * kSsmTile;
     float *h_ = y_ + p.cw * kSsmTile, *A_ = h_ + p.cw * p.NP;
     const int len = ssm_length(p, w.b);
     const int64_t row0 = w.b * p.channels + w.d0;
+    const S *xrow = p.x + w.b * p.xs[0] + w.d0 * p.xs[1], *drow = p.delta + w.b * p.ds[0] + w.d0 * p.ds[1];
+    const S *zrow = p.z ? p.z + w.b * p.zs[0] + w.d0 * p.zs[1] : nullptr;
+    const S *Brow = p.B + w.b * p.Bs[0] + w.g * p.Bs[1], *Crow = p.C + w.b * p.Cs[0] + w.g * p.Cs[1];
 
-    for (int i = lane; i < w.nc * p.NP; i += 32) {
-        const int c = i / p.NP, n = i - c * p.NP;
-        A_[i] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
-        h_[i] = n < p.N && p.h0 ? p.h0[(row0 + c) * p.N + n] : 0.f;
-    }
-    __syncwarp();
+    for (int c = 0; c < w.nc; ++c)
+        for (int n = lane; n < p.NP; n += 32) {
+            A_[c * p.NP + n] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
+            h_[c * p.NP + n] = n < p.N && p.h0 ? p.h0[(row0 + c) * p.N + n] : 0.f;
+        }
 
-    for (int tile = 0; tile < p.tiles; ++tile) {
-        const int t = tile * kSsmTile + s * kSsmE;
-        if (tile * kSsmTile >= len) {  // behind the sequence: zeros
-            const float zero[8] = {};
-            for (int c = q; c < w.nc; c += 4) store8<S, ALIGNED>(out + (row0 + c) * p.T, t, p.T, zero);
-            continue;
-        }
-        if (checkpoints) {
-            float *ck = checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
-            for (int i = lane; i < w.nc * p.N; i += 32) ck[i] = h_[i / p.N * p.NP + i % p.N];
-        }
-        for (int c = q; c < w.nc; c += 4) {
-            float x[8], dt[8];
-            load8<S, ALIGNED>(p.x + w.b * p.xs[0] + (w.d0 + c) * p.xs[1], t, len, x);
-            load8<S, ALIGNED>(p.delta + w.b * p.ds[0] + (w.d0 + c) * p.ds[1], t, len, dt);
-            time_steps(p, p.bias ? p.bias[w.d0 + c] : 0.f, t, len, dt);
-            tile_put(dt_ + c * kSsmTile, s, dt);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= dt[i];
-            tile_put(u_ + c * kSsmTile, s, x);
-        }
-        __syncwarp();
+    const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
+    const int kinds = p.z ? 3 : 2;
+    const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
+    auto stage = [&](int tile, int nb, int step) {
+        const int t0 = tile * kSsmTile;
+        stage_rows<S, ALIGNED>(ssm_smem + (step & 1) * (2 * kSsmNB * RB), 2 * kSsmNB, t0, len, threadIdx.x,
+                               kSsmFwdWarps * 32, any, [&](int r) -> const S * {
+                                   const int n = nb * kSsmNB + (r & (kSsmNB - 1));
+                                   return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
+                               });
+        if (nb == 0)
+            stage_rows<S, ALIGNED>(raw + (tile & 1) * (3 * p.cw * RB), w.nc * kinds, t0, len, lane, 32, any, [&](int r) -> const S * {
+                const int kind = r / w.nc, c = r - kind * w.nc;  // rows: x of every channel, then delta, then z
+                return kind == 0 ? xrow + c * p.xs[1] : kind == 1 ? drow + c * p.ds[1] : zrow + c * p.zs[1];
+            });
+        copies_commit();
+    };
+    if (live_tiles > 0) stage(0, 0, 0);
 
-        for (int n0 = q * kSsmNL; n0 < p.NP; n0 += kSsmNB) {
-            float B[kSsmNL][8], C[kSsmNL][8];
-#pragma unroll
-            for (int j = 0; j < kSsmNL; ++j) {
-                const int lim = n0 + j < p.N ? len : 0;
-                load8<S, ALIGNED>(p.B + w.b * p.Bs[0] + w.g * p.Bs[1] + (n0 + j) * p.Bs[2], t, lim, B[j]);
-                load8<S, ALIGNED>(p.C + w.b * p.Cs[0] + w.g * p.Cs[1] + (n0 + j) * p.Cs[2], t, lim, C[j]);
-            }
-            for (int c = 0; c < w.nc; ++c) {
-                float dt[8], u[8], y[8], sum = 0.f;
-                tile_get(dt_ + c * kSsmTile, s, dt);
-                tile_get(u_ + c * kSsmTile, s, u);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum += dt[i];
-                    y[i] = 0.f;
+    for (int tile = 0, step = 0; tile < live_tiles; ++tile) {
+        const int t = tile * kSsmTile + 2 * lane;  // this lane's two positions outside the state loop
+        const unsigned char *mine = raw + (tile & 1) * (3 * p.cw * RB);
+        for (int nb = 0; nb < blocks; ++nb, ++step) {
+            copies_wait();
+            __syncthreads();
+            if (nb + 1 < blocks) stage(tile, nb + 1, step + 1);
+            else if (tile + 1 < live_tiles) stage(tile + 1, 0, step + 1);
+            if (nb == 0) {
+                for (int c = 0; c < w.nc; ++c) {
+                    const float bias = p.bias ? p.bias[w.d0 + c] : 0.f;
+                    const float2 x = row_pair<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), lane);
+                    const float2 r = row_pair<S, ALIGNED>(mine + (w.nc + c) * RB, row_shift<S, ALIGNED>(drow + c * p.ds[1]), lane);
+                    const float2 dt = make_float2(time_step(r.x, bias, p.softplus, t < len),
+                                                  time_step(r.y, bias, p.softplus, t + 1 < len));
+                    *reinterpret_cast<float2 *>(dt_ + c * kSsmTile + pair_at(lane)) = dt;
+                    *reinterpret_cast<float2 *>(u_ + c * kSsmTile + pair_at(lane)) = make_float2(dt.x * x.x, dt.y * x.y);
                 }
+                if (checkpoints) {
+                    float *ck = checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
+                    for (int c = 0; c < w.nc; ++c)
+                        for (int n = lane; n < p.N; n += 32) ck[c * p.N + n] = h_[c * p.NP + n];
+                }
+                __syncwarp();
+            }
+            const int n0 = nb * kSsmNB + q * kSsmNL;
+            f2 B[kSsmNL][4], C[kSsmNL][4];
+            {
+                const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
 #pragma unroll
                 for (int j = 0; j < kSsmNL; ++j) {
-                    const float A = A_[c * p.NP + n0 + j], carry = h_[c * p.NP + n0 + j];
-                    float a[8], S0 = 0.f;
+                    const int r = q * kSsmNL + j;
+                    row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(Brow + (n0 + j) * p.Bs[2]), s, B[j]);
+                    row_eight<S, ALIGNED>(bc + (kSsmNB + r) * RB, row_shift<S, ALIGNED>(Crow + (n0 + j) * p.Cs[2]), s, C[j]);
+                }
+            }
+            for (int c = 0; c < w.nc; ++c) {
+                f2 dt[4], u[4], y[4];
+                tile_get(dt_ + c * kSsmTile, s, dt);
+                tile_get(u_ + c * kSsmTile, s, u);
+                const float4 A4 = *reinterpret_cast<const float4 *>(A_ + c * p.NP + n0);
+                float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
+                __syncwarp();  // the carries are read before the last time lane replaces them
+                const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
+                float hv[4] = {h4.x, h4.y, h4.z, h4.w};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        a[i] = ex2(dt[i] * A);
-                        S0 = fmaf(a[i], S0, u[i] * B[j][i]);
+                for (int k = 0; k < 4; ++k) y[k] = 0;
+#pragma unroll
+                for (int j = 0; j < kSsmNL; ++j) {
+                    const f2 Ad = pk(Av[j], Av[j]);
+                    f2 a[4], b[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const f2 e = mul2(dt[k], Ad);
+                        a[k] = pk(ex2(lo(e)), ex2(hi(e)));
+                        b[k] = mul2(u[k], B[j][k]);
                     }
-                    const float P = ex2(sum * A);
-                    if (s == 0) S0 = fmaf(P, carry, S0);
-                    S0 = scan_up(P, S0, s);
-                    float h = __shfl_up_sync(kFullMask, S0, 1, 8);
-                    if (s == 0) h = carry;
-                    if (s == 7) h_[c * p.NP + n0 + j] = S0;
+                    float S0 = lo(b[0]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        h = fmaf(a[i], h, u[i] * B[j][i]);
-                        y[i] = fmaf(C[j][i], h, y[i]);
+                    for (int k = 0; k < 4; ++k) {
+                        if (k) S0 = fmaf(lo(a[k]), S0, lo(b[k]));
+                        S0 = fmaf(hi(a[k]), S0, hi(b[k]));
+                    }
+                    float h = lane_scan<true>(product8(a), S0, hv[j], s);
+                    hv[j] = S0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float h1 = fmaf(lo(a[k]), h, lo(b[k]));
+                        h = fmaf(hi(a[k]), h1, hi(b[k]));
+                        y[k] = fma2(C[j][k], pk(h1, h), y[k]);
                     }
                 }
-                tile_sum(y_ + c * kSsmTile, s, q, y, n0 < kSsmNB);
+                if (s == 7) *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+                tile_sum(y_ + c * kSsmTile, s, q, y, nb == 0);
             }
         }
         __syncwarp();
-
-        for (int c = q; c < w.nc; c += 4) {
-            float y[8], x[8];
-            tile_get(y_ + c * kSsmTile, s, y);
+        for (int c = 0; c < w.nc; ++c) {
+            float2 y = *reinterpret_cast<const float2 *>(y_ + c * kSsmTile + pair_at(lane));
             if (p.D) {
                 const float D = p.D[w.d0 + c];
-                load8<S, ALIGNED>(p.x + w.b * p.xs[0] + (w.d0 + c) * p.xs[1], t, len, x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = fmaf(D, x[i], y[i]);
+                const float2 x = row_pair<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), lane);
+                y = make_float2(fmaf(D, x.x, y.x), fmaf(D, x.y, y.y));
             }
             if (p.z) {
-                float z[8];
-                load8<S, ALIGNED>(p.z + w.b * p.zs[0] + (w.d0 + c) * p.zs[1], t, len, z);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= z[i] * sigmoid_f(z[i]);
+                const float2 z = row_pair<S, ALIGNED>(mine + (2 * w.nc + c) * RB, row_shift<S, ALIGNED>(zrow + c * p.zs[1]), lane);
+                y = make_float2(y.x * z.x * sigmoid_f(z.x), y.y * z.y * sigmoid_f(z.y));
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = t + i < len ? y[i] : 0.f;
-            store8<S, ALIGNED>(out + (row0 + c) * p.T, t, p.T, y);
+            store_pair<S, ALIGNED>(out + (row0 + c) * p.T, t, p.T, t < len ? y.x : 0.f, t + 1 < len ? y.y : 0.f);
         }
-        __syncwarp();
     }
+    __syncwarp();
+    for (int tile = live_tiles; tile < p.tiles; ++tile)  // behind the sequence: zeros
+        for (int c = 0; c < w.nc; ++c)
+            store_pair<S, ALIGNED>(out + (row0 + c) * p.T, tile * kSsmTile + 2 * lane, p.T, 0.f, 0.f);
     if (h_last)
-        for (int i = lane; i < w.nc * p.N; i += 32) h_last[row0 * p.N + i] = h_[i / p.N * p.NP + i % p.N];
+        for (int c = 0; c < w.nc; ++c)
+            for (int n = lane; n < p.N; n += 32) h_last[(row0 + c) * p.N + n] = h_[c * p.NP + n];
 }
 
 // What the backward writes; the partial sums live in the caller's workspace.
@@ -334,7 +497,8 @@ struct SsmGrads {
     float *d_part;   // [batch][2][D]: grad of D, grad of delta_bias
 };
 
-// g_t = C_t dy_t + c_{t+1},  c_t = a_t g_t;  with q_t = c_t h_{t-1}:
+// With e_t = C_t dy_t:  c_t = a_t (e_t + c_{t+1}) is what reaches the state before t, g_t = e_t + c_{t+1},
+// q_t = c_t h_{t-1};
 //   ddt_t = sum_n A q_t + x_t sum_n g_t B_t,  dx_t = dt_t sum_n g_t B_t + D dy_t,
 //   dA = sum_t dt_t q_t,  dB_t = sum_d g_t u_t,  dC_t = sum_d dy_t h_t.
 // The tiles are walked from the last to the first; the states of a tile are recomputed in registers
@@ -345,156 +509,207 @@ struct SsmGrads {
 template <typename S, bool ALIGNED, bool GATED>
 __global__ void __launch_bounds__(kSsmBwdWarps * 32, 1)
 ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
-    extern __shared__ __align__(16) float ssm_smem[];
-    constexpr int W = kSsmBwdWarps;
+    extern __shared__ __align__(16) unsigned char ssm_smem[];
+    constexpr int W = kSsmBwdWarps, RB = row_bytes<S>(), kinds = GATED ? 4 : 3;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3;
     const SsmPlace w = ssm_place(p, W);
-    float *red = ssm_smem;  // [warp][64][lane]
-    float *dt_ = red + W * 64 * 32 + warp * ssm_bwd_floats(p.cw, p.NP);
+    float *red = reinterpret_cast<float *>(ssm_smem + ssm_bc_bytes<S>());  // [warp][64][lane]
+    unsigned char *raw = reinterpret_cast<unsigned char *>(red + W * 64 * 32) + warp * ssm_bwd_warp_bytes<S>(p.cw, p.NP);
     const int ct = p.cw * kSsmTile, cn = p.cw * p.NP;
+    float *dt_ = reinterpret_cast<float *>(raw + 2 * 4 * p.cw * RB);
     float *u_ = dt_ + ct, *dy_ = u_ + ct, *gB_ = dy_ + ct, *q_ = gB_ + ct, *y_ = q_ + ct;
     float *A_ = y_ + ct, *h_ = A_ + cn, *c_ = h_ + cn, *dA_ = c_ + cn, *dD_ = dA_ + cn, *db_ = dD_ + p.cw;
     const int len = ssm_length(p, w.b);
     const int64_t row0 = w.b * p.channels + w.d0;
     const int Tpad = p.tiles * kSsmTile;
-    float *bc = o.bc_part + ((w.b * p.groups + w.g) * p.chunks + w.chunk) * 2 * p.N * static_cast<int64_t>(Tpad);
+    float *bc_out = o.bc_part + ((w.b * p.groups + w.g) * p.chunks + w.chunk) * 2 * p.N * static_cast<int64_t>(Tpad);
+    const S *xrow = p.x + w.b * p.xs[0] + w.d0 * p.xs[1], *drow = p.delta + w.b * p.ds[0] + w.d0 * p.ds[1];
+    const S *zrow = GATED ? p.z + w.b * p.zs[0] + w.d0 * p.zs[1] : nullptr, *grow = o.grad_out + row0 * p.T;
+    const S *Brow = p.B + w.b * p.Bs[0] + w.g * p.Bs[1], *Crow = p.C + w.b * p.Cs[0] + w.g * p.Cs[1];
 
-    for (int i = lane; i < w.nc * p.NP; i += 32) {
-        const int c = i / p.NP, n = i - c * p.NP;
-        A_[i] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
-        c_[i] = n < p.N && o.grad_last ? o.grad_last[(row0 + c) * p.N + n] : 0.f;
-        h_[i] = 0.f;
-        dA_[i] = 0.f;
+    for (int c = 0; c < w.nc; ++c) {
+        for (int n = lane; n < p.NP; n += 32) {
+            const int i = c * p.NP + n;
+            A_[i] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
+            c_[i] = n < p.N && o.grad_last ? o.grad_last[(row0 + c) * p.N + n] : 0.f;
+            h_[i] = 0.f;
+            dA_[i] = 0.f;
+        }
+        if (lane == 0) dD_[c] = db_[c] = 0.f;
     }
-    for (int i = lane; i < w.nc; i += 32) dD_[i] = db_[i] = 0.f;
 
-    for (int tile = p.tiles - 1; tile >= 0; --tile) {
-        const int t = tile * kSsmTile + s * kSsmE;
-        if (tile * kSsmTile >= len) {
-            const float zero[8] = {};
-            for (int c = q; c < w.nc; c += 4) {
-                store8<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, zero);
-                store8<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, zero);
-                if (GATED) store8<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T, zero);
-            }
-            for (int i = threadIdx.x; i < 2 * p.N * kSsmTile; i += W * 32)
-                bc[static_cast<int64_t>(i / kSsmTile) * Tpad + tile * kSsmTile + i % kSsmTile] = 0.f;
-            continue;
-        }
-        __syncwarp();
-        {
-            const float *ck = o.checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
-            for (int i = lane; i < w.nc * p.N; i += 32) h_[i / p.N * p.NP + i % p.N] = ck[i];
-        }
-        for (int c = q; c < w.nc; c += 4) {
-            float x[8], dt[8], dy[8];
-            load8<S, ALIGNED>(p.x + w.b * p.xs[0] + (w.d0 + c) * p.xs[1], t, len, x);
-            load8<S, ALIGNED>(p.delta + w.b * p.ds[0] + (w.d0 + c) * p.ds[1], t, len, dt);
-            load8<S, ALIGNED>(o.grad_out + (row0 + c) * p.T, t, len, dy);
-            time_steps(p, p.bias ? p.bias[w.d0 + c] : 0.f, t, len, dt);
-            if (GATED) {
-                float z[8];
-                load8<S, ALIGNED>(p.z + w.b * p.zs[0] + (w.d0 + c) * p.zs[1], t, len, z);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dy[i] = t + i < len ? dy[i] * z[i] * sigmoid_f(z[i]) : 0.f;
-            }
-            tile_put(dt_ + c * kSsmTile, s, dt);
-            tile_put(dy_ + c * kSsmTile, s, dy);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= dt[i];
-            tile_put(u_ + c * kSsmTile, s, x);
-        }
-        __syncwarp();
+    const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
+    const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
+    auto stage = [&](int tile, int nb, int step) {
+        const int t0 = tile * kSsmTile;
+        stage_rows<S, ALIGNED>(ssm_smem + (step & 1) * (2 * kSsmNB * RB), 2 * kSsmNB, t0, len, threadIdx.x, W * 32, any,
+                               [&](int r) -> const S * {
+                                   const int n = nb * kSsmNB + (r & (kSsmNB - 1));
+                                   return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
+                               });
+        if (nb == 0)
+            stage_rows<S, ALIGNED>(raw + (tile & 1) * (4 * p.cw * RB), w.nc * kinds, t0, len, lane, 32, any, [&](int r) -> const S * {
+                const int kind = r / w.nc, c = r - kind * w.nc;  // rows: x of every channel, then delta, grad_out, z
+                return kind == 0   ? xrow + c * p.xs[1]
+                       : kind == 1 ? drow + c * p.ds[1]
+                       : kind == 2 ? grow + static_cast<int64_t>(c) * p.T
+                                   : zrow + c * p.zs[1];
+            });
+        copies_commit();
+    };
+    auto row_at = [&](const unsigned char *mine, int kind, int c) {
+        const S *first = kind == 0   ? xrow + c * p.xs[1]
+                         : kind == 1 ? drow + c * p.ds[1]
+                         : kind == 2 ? grow + static_cast<int64_t>(c) * p.T
+                                     : zrow + c * p.zs[1];
+        return row_pair<S, ALIGNED>(mine + (kind * w.nc + c) * RB, row_shift<S, ALIGNED>(first), lane);
+    };
 
-        for (int nb = 0; nb < p.NP; nb += kSsmNB) {
-            const int n0 = nb + q * kSsmNL;
-            float B[kSsmNL][8], C[kSsmNL][8], dB[kSsmNL][8], dC[kSsmNL][8];
+    for (int tile = p.tiles - 1; tile >= live_tiles; --tile) {  // behind the sequence: zeros
+        const int t = tile * kSsmTile + 2 * lane;
+        for (int c = 0; c < w.nc; ++c) {
+            store_pair<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
+            store_pair<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
+            if (GATED) store_pair<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
+        }
+        for (int i = threadIdx.x; i < 2 * p.N * kSsmTile; i += W * 32)
+            bc_out[static_cast<int64_t>(i / kSsmTile) * Tpad + tile * kSsmTile + i % kSsmTile] = 0.f;
+    }
+    if (live_tiles > 0) stage(live_tiles - 1, 0, 0);
+
+    for (int tile = live_tiles - 1, step = 0; tile >= 0; --tile) {
+        const int t = tile * kSsmTile + 2 * lane;
+        const unsigned char *mine = raw + (tile & 1) * (4 * p.cw * RB);
+        for (int nb = 0; nb < blocks; ++nb, ++step) {
+            copies_wait();
+            __syncthreads();
+            if (nb + 1 < blocks) stage(tile, nb + 1, step + 1);
+            else if (tile > 0) stage(tile - 1, 0, step + 1);
+            if (nb == 0) {
+                const float *ck = o.checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
+                for (int c = 0; c < w.nc; ++c) {
+                    for (int n = lane; n < p.N; n += 32) h_[c * p.NP + n] = ck[c * p.N + n];
+                    const float bias = p.bias ? p.bias[w.d0 + c] : 0.f;
+                    const float2 x = row_at(mine, 0, c), r = row_at(mine, 1, c);
+                    float2 dy = row_at(mine, 2, c);
+                    if (GATED) {
+                        const float2 z = row_at(mine, 3, c);
+                        dy = make_float2(dy.x * z.x * sigmoid_f(z.x), dy.y * z.y * sigmoid_f(z.y));
+                    }
+                    const float2 dt = make_float2(time_step(r.x, bias, p.softplus, t < len),
+                                                  time_step(r.y, bias, p.softplus, t + 1 < len));
+                    const int at = c * kSsmTile + pair_at(lane);
+                    *reinterpret_cast<float2 *>(dt_ + at) = dt;
+                    *reinterpret_cast<float2 *>(u_ + at) = make_float2(dt.x * x.x, dt.y * x.y);
+                    *reinterpret_cast<float2 *>(dy_ + at) = dy;
+                }
+                __syncwarp();
+            }
+            const int n0 = nb * kSsmNB + q * kSsmNL;
+            f2 B[kSsmNL][4], C[kSsmNL][4], dB[kSsmNL][4], dC[kSsmNL][4];
+            {
+                const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
 #pragma unroll
-            for (int j = 0; j < kSsmNL; ++j) {
-                const int lim = n0 + j < p.N ? len : 0;
-                load8<S, ALIGNED>(p.B + w.b * p.Bs[0] + w.g * p.Bs[1] + (n0 + j) * p.Bs[2], t, lim, B[j]);
-                load8<S, ALIGNED>(p.C + w.b * p.Cs[0] + w.g * p.Cs[1] + (n0 + j) * p.Cs[2], t, lim, C[j]);
+                for (int j = 0; j < kSsmNL; ++j) {
+                    const int r = q * kSsmNL + j;
+                    row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(Brow + (n0 + j) * p.Bs[2]), s, B[j]);
+                    row_eight<S, ALIGNED>(bc + (kSsmNB + r) * RB, row_shift<S, ALIGNED>(Crow + (n0 + j) * p.Cs[2]), s, C[j]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dB[j][i] = dC[j][i] = 0.f;
+                    for (int k = 0; k < 4; ++k) dB[j][k] = dC[j][k] = 0;
+                }
             }
             for (int c = 0; c < w.nc; ++c) {
-                float dt[8], u[8], dy[8], gB[8], Q[8], y[8], dA[kSsmNL], sum = 0.f;
+                f2 dt[4], u[4], dy[4], gB[4], Q[4], y[4];
+                float dA[kSsmNL];
                 tile_get(dt_ + c * kSsmTile, s, dt);
                 tile_get(u_ + c * kSsmTile, s, u);
                 tile_get(dy_ + c * kSsmTile, s, dy);
+                const int at = c * p.NP + n0;
+                const float4 A4 = *reinterpret_cast<const float4 *>(A_ + at), h4 = *reinterpret_cast<const float4 *>(h_ + at);
+                const float4 c4 = *reinterpret_cast<const float4 *>(c_ + at);
+                __syncwarp();  // the carries are read before the first time lane replaces them
+                const float Av[4] = {A4.x, A4.y, A4.z, A4.w}, hv[4] = {h4.x, h4.y, h4.z, h4.w};
+                float cv[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum += dt[i];
-                    gB[i] = Q[i] = y[i] = 0.f;
-                }
+                for (int k = 0; k < 4; ++k) gB[k] = Q[k] = y[k] = 0;
 #pragma unroll
                 for (int j = 0; j < kSsmNL; ++j) {
-                    const int at = c * p.NP + n0 + j;
-                    const float A = A_[at], first = h_[at], carry = c_[at];
-                    float a[8], h[8], S0 = 0.f;
+                    const f2 Ad = pk(Av[j], Av[j]);
+                    f2 a[4], v[4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        a[i] = ex2(dt[i] * A);
-                        S0 = fmaf(a[i], S0, u[i] * B[j][i]);
+                    for (int k = 0; k < 4; ++k) {
+                        const f2 x = mul2(dt[k], Ad);
+                        a[k] = pk(ex2(lo(x)), ex2(hi(x)));
+                        v[k] = mul2(u[k], B[j][k]);
                     }
-                    const float P = ex2(sum * A);
-                    if (s == 0) S0 = fmaf(P, first, S0);
-                    S0 = scan_up(P, S0, s);
-                    float hin = __shfl_up_sync(kFullMask, S0, 1, 8);
-                    if (s == 0) hin = first;
-                    float R0 = 0.f;
+                    float S0 = lo(v[0]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        h[i] = fmaf(a[i], i ? h[i - 1] : hin, u[i] * B[j][i]);
-                        dC[j][i] = fmaf(dy[i], h[i], dC[j][i]);
-                        if (GATED) y[i] = fmaf(C[j][i], h[i], y[i]);
+                    for (int k = 0; k < 4; ++k) {
+                        if (k) S0 = fmaf(lo(a[k]), S0, lo(v[k]));
+                        S0 = fmaf(hi(a[k]), S0, hi(v[k]));
                     }
+                    const float P = product8(a);
+                    const float hin = lane_scan<true>(P, S0, hv[j], s);
+                    f2 h[4], e[4];
 #pragma unroll
-                    for (int i = 7; i >= 0; --i) R0 = a[i] * fmaf(C[j][i], dy[i], R0);
-                    if (s == 7) R0 = fmaf(P, carry, R0);
-                    R0 = scan_down(P, R0, s);
-                    float cc = __shfl_down_sync(kFullMask, R0, 1, 8);
-                    if (s == 7) cc = carry;
-                    if (s == 0) c_[at] = R0;
-                    dA[j] = 0.f;
-#pragma unroll
-                    for (int i = 7; i >= 0; --i) {
-                        const float g = fmaf(C[j][i], dy[i], cc);
-                        cc = a[i] * g;
-                        const float qq = cc * (i ? h[i - 1] : hin);
-                        Q[i] = fmaf(A, qq, Q[i]);
-                        dA[j] = fmaf(dt[i], qq, dA[j]);
-                        gB[i] = fmaf(g, B[j][i], gB[i]);
-                        dB[j][i] = fmaf(g, u[i], dB[j][i]);
+                    for (int k = 0; k < 4; ++k) {
+                        const float h1 = fmaf(lo(a[k]), k ? hi(h[k ? k - 1 : 0]) : hin, lo(v[k]));
+                        h[k] = pk(h1, fmaf(hi(a[k]), h1, hi(v[k])));
+                        dC[j][k] = fma2(dy[k], h[k], dC[j][k]);
+                        if (GATED) y[k] = fma2(C[j][k], h[k], y[k]);
+                        e[k] = mul2(C[j][k], dy[k]);
+                        v[k] = mul2(a[k], e[k]);
                     }
+                    float R0 = hi(v[3]);
+#pragma unroll
+                    for (int k = 3; k >= 0; --k) {
+                        if (k < 3) R0 = fmaf(hi(a[k]), R0, hi(v[k]));
+                        R0 = fmaf(lo(a[k]), R0, lo(v[k]));
+                    }
+                    float after = lane_scan<false>(P, R0, cv[j], s);  // c of the position behind
+                    cv[j] = R0;
+                    f2 dAj = 0;
+#pragma unroll
+                    for (int k = 3; k >= 0; --k) {
+                        const float c1 = fmaf(hi(a[k]), after, hi(v[k])), c0 = fmaf(lo(a[k]), c1, lo(v[k]));
+                        const f2 g = add2(e[k], pk(c1, after));
+                        const f2 qq = pk(c0 * (k ? hi(h[k ? k - 1 : 0]) : hin), c1 * lo(h[k]));
+                        after = c0;
+                        Q[k] = fma2(Ad, qq, Q[k]);
+                        dAj = fma2(dt[k], qq, dAj);
+                        gB[k] = fma2(g, B[j][k], gB[k]);
+                        dB[j][k] = fma2(g, u[k], dB[j][k]);
+                    }
+                    dA[j] = lo(dAj) + hi(dAj);
                 }
+                if (s == 0) *reinterpret_cast<float4 *>(c_ + at) = make_float4(cv[0], cv[1], cv[2], cv[3]);
                 {  // dA over the 8 time lanes: lane s < 4 keeps state 2 * (s & 1) + (s >> 1)
-                    const bool hi = s & 1, hi2 = s & 2;
-                    const float k0 = hi ? dA[2] : dA[0], g0 = hi ? dA[0] : dA[2];
-                    const float k1 = hi ? dA[3] : dA[1], g1 = hi ? dA[1] : dA[3];
-                    const float r0 = k0 + __shfl_xor_sync(kFullMask, g0, 1);
-                    const float r1 = k1 + __shfl_xor_sync(kFullMask, g1, 1);
-                    float v = (hi2 ? r1 : r0) + __shfl_xor_sync(kFullMask, hi2 ? r0 : r1, 2);
-                    v += __shfl_xor_sync(kFullMask, v, 4);
-                    if (s < 4) dA_[c * p.NP + n0 + 2 * (s & 1) + (s >> 1)] += v;
+                    const bool up = s & 1, up2 = s & 2;
+                    const float r0 = (up ? dA[2] : dA[0]) + __shfl_xor_sync(kFullMask, up ? dA[0] : dA[2], 1);
+                    const float r1 = (up ? dA[3] : dA[1]) + __shfl_xor_sync(kFullMask, up ? dA[1] : dA[3], 1);
+                    float d = (up2 ? r1 : r0) + __shfl_xor_sync(kFullMask, up2 ? r0 : r1, 2);
+                    d += __shfl_xor_sync(kFullMask, d, 4);
+                    if (s < 4) dA_[at + 2 * (s & 1) + (s >> 1)] += d;
                 }
                 tile_sum(gB_ + c * kSsmTile, s, q, gB, nb == 0);
                 tile_sum(q_ + c * kSsmTile, s, q, Q, nb == 0);
                 if (GATED) tile_sum(y_ + c * kSsmTile, s, q, y, nb == 0);
             }
             // dB, dC over the warps of the CTA
-            float *mine = red + warp * 64 * 32 + lane;
+            float *slot = red + warp * 64 * 32 + lane;
 #pragma unroll
             for (int j = 0; j < kSsmNL; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    mine[(j * 8 + i) * 32] = dB[j][i];
-                    mine[((4 + j) * 8 + i) * 32] = dC[j][i];
+                for (int k = 0; k < 4; ++k) {
+                    slot[(j * 8 + 2 * k) * 32] = lo(dB[j][k]);
+                    slot[(j * 8 + 2 * k + 1) * 32] = hi(dB[j][k]);
+                    slot[((4 + j) * 8 + 2 * k) * 32] = lo(dC[j][k]);
+                    slot[((4 + j) * 8 + 2 * k + 1) * 32] = hi(dC[j][k]);
                 }
             __syncthreads();
             {
                 static_assert(W == 2 * kSsmNL, "a warp sums the values of one state of dB or dC");
-                const int n = nb + q * kSsmNL + (warp & 3);
+                const int n = n0 + (warp & 3);
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -503,72 +718,58 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                     for (int k = 0; k < W; ++k) v[i] += red[(k * 64 + warp * 8 + i) * 32 + lane];
                 }
                 if (n < p.N) {
-                    float4 *to = reinterpret_cast<float4 *>(bc + (static_cast<int64_t>(warp >> 2) * p.N + n) * Tpad + t);
+                    float4 *to = reinterpret_cast<float4 *>(bc_out + (static_cast<int64_t>(warp >> 2) * p.N + n) * Tpad +
+                                                            tile * kSsmTile + s * kSsmE);
                     to[0] = make_float4(v[0], v[1], v[2], v[3]);
                     to[1] = make_float4(v[4], v[5], v[6], v[7]);
                 }
             }
-            __syncthreads();
         }
 
-        for (int c = q; c < w.nc; c += 4) {
-            float x[8], raw[8], dy[8], dt[8], gB[8], Q[8], out[8];
-            tile_get(dt_ + c * kSsmTile, s, dt);
-            tile_get(dy_ + c * kSsmTile, s, dy);
-            tile_get(gB_ + c * kSsmTile, s, gB);
-            tile_get(q_ + c * kSsmTile, s, Q);
+        for (int c = 0; c < w.nc; ++c) {
+            const int at = c * kSsmTile + pair_at(lane);
+            const float2 dt = *reinterpret_cast<const float2 *>(dt_ + at), dy = *reinterpret_cast<const float2 *>(dy_ + at);
+            const float2 gB = *reinterpret_cast<const float2 *>(gB_ + at), Q = *reinterpret_cast<const float2 *>(q_ + at);
             const float D = p.D ? p.D[w.d0 + c] : 0.f, bias = p.bias ? p.bias[w.d0 + c] : 0.f;
-            load8<S, ALIGNED>(p.x + w.b * p.xs[0] + (w.d0 + c) * p.xs[1], t, len, x);
-            load8<S, ALIGNED>(p.delta + w.b * p.ds[0] + (w.d0 + c) * p.ds[1], t, len, raw);
-            float sD = 0.f, sb = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                out[i] = t + i < len ? fmaf(dt[i], gB[i], D * dy[i]) : 0.f;
-                sD = fmaf(dy[i], x[i], sD);
-            }
-            store8<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, out);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float v = fmaf(kLn2, Q[i], x[i] * gB[i]);
-                if (p.softplus && raw[i] + bias <= 20.f) v *= sigmoid_f(raw[i] + bias);
-                out[i] = t + i < len ? v : 0.f;
-                sb += out[i];
-            }
-            store8<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, out);
+            const float2 x = row_at(mine, 0, c), r = row_at(mine, 1, c);
+            const bool on0 = t < len, on1 = t + 1 < len;
+            store_pair<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, on0 ? fmaf(dt.x, gB.x, D * dy.x) : 0.f,
+                                   on1 ? fmaf(dt.y, gB.y, D * dy.y) : 0.f);
+            float2 d = make_float2(fmaf(kLn2, Q.x, x.x * gB.x), fmaf(kLn2, Q.y, x.y * gB.y));
+            if (p.softplus) d = make_float2(d.x * sigmoid_f(r.x + bias), d.y * sigmoid_f(r.y + bias));
+            d = make_float2(on0 ? d.x : 0.f, on1 ? d.y : 0.f);
+            store_pair<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, d.x, d.y);
             if (GATED) {
-                float z[8], y[8], up[8];
-                tile_get(y_ + c * kSsmTile, s, y);
-                load8<S, ALIGNED>(p.z + w.b * p.zs[0] + (w.d0 + c) * p.zs[1], t, len, z);
-                load8<S, ALIGNED>(o.grad_out + (row0 + c) * p.T, t, len, up);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float sg = sigmoid_f(z[i]);
-                    out[i] = t + i < len ? up[i] * fmaf(D, x[i], y[i]) * sg * fmaf(z[i], 1.f - sg, 1.f) : 0.f;
-                }
-                store8<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T, out);
+                const float2 y = *reinterpret_cast<const float2 *>(y_ + at);
+                const float2 z = row_at(mine, 3, c), up = row_at(mine, 2, c);
+                const float g0 = sigmoid_f(z.x), g1 = sigmoid_f(z.y);
+                store_pair<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T,
+                                       on0 ? up.x * fmaf(D, x.x, y.x) * g0 * fmaf(z.x, 1.f - g0, 1.f) : 0.f,
+                                       on1 ? up.y * fmaf(D, x.y, y.y) * g1 * fmaf(z.y, 1.f - g1, 1.f) : 0.f);
             }
-            // the lanes of one state-lane row hold one channel: they are the active ones
-            const unsigned row = 0xffu << (q * 8);
+            float sD = fmaf(dy.x, x.x, dy.y * x.y), sb = d.x + d.y;
 #pragma unroll
-            for (int k = 1; k < 8; k *= 2) {
-                sD += __shfl_xor_sync(row, sD, k);
-                sb += __shfl_xor_sync(row, sb, k);
+            for (int k = 1; k < 32; k *= 2) {
+                sD += __shfl_xor_sync(kFullMask, sD, k);
+                sb += __shfl_xor_sync(kFullMask, sb, k);
             }
-            if (s == 0) {
+            if (lane == 0) {
                 dD_[c] += sD;
                 db_[c] += sb;
             }
         }
     }
     __syncwarp();
-    for (int i = lane; i < w.nc * p.N; i += 32) {
-        const int c = i / p.N, k = c * p.NP + i % p.N;
-        o.a_part[row0 * p.N + i] = dA_[k];
-        if (o.dh0) o.dh0[row0 * p.N + i] = c_[k];
-    }
-    for (int i = lane; i < w.nc; i += 32) {
-        o.d_part[(w.b * 2) * p.channels + w.d0 + i] = dD_[i];
-        o.d_part[(w.b * 2 + 1) * p.channels + w.d0 + i] = db_[i];
+    for (int c = 0; c < w.nc; ++c) {
+        for (int n = lane; n < p.N; n += 32) {
+            const int k = c * p.NP + n;
+            o.a_part[(row0 + c) * p.N + n] = dA_[k];
+            if (o.dh0) o.dh0[(row0 + c) * p.N + n] = c_[k];
+        }
+        if (lane == 0) {
+            o.d_part[(w.b * 2) * p.channels + w.d0 + c] = dD_[c];
+            o.d_part[(w.b * 2 + 1) * p.channels + w.d0 + c] = db_[c];
+        }
     }
 }
 

@@ -4,10 +4,10 @@ Tolerances.  A stored value is off by half a step of its type, ``eps / 2`` relat
 evaluation in front of it is a sum of products; each product's relative error is at most the number of
 roundings on its path times 2^-24, so the sum is off by that count times the sum of the absolute values
 (``magnitude=True`` of the reference).  A path runs through at most T decays (backward: twice).  One
-decay exp(dt A) takes its argument with 5 roundings (the time step 3, A log2(e) and the product one
-each), which the exponential turns into 5 |dt A| relative, and comes out of the exponential within
-2^-22, 4 roundings, and is multiplied with one: 5 |dt A| + 5 per position, and 3 for the position's own
-products.  Sums over states, channels, positions and sequences add one rounding a term.  The gate and the
+decay exp(dt A) takes its argument with 20 roundings: A log2(e) and the product one each, and the time
+step log(1 + exp(v)), |v| <= 8 here, 18: its exponential |v| from the argument and 4 of its own, the
+quotient 3, the series 3.  The exponential turns them into 20 |dt A| relative, adds 2^-22, 4 roundings,
+and the multiplication one: 20 |dt A| + 5 per position, and 3 for the position's own products.  Sums over states, channels, positions and sequences add one rounding a term.  The gate and the
 time step add 64 (|z| <= 6: argument 2 |z| + 1, exponential 4, division 4; the same for softplus).
 """
 import numpy as np
@@ -68,7 +68,7 @@ def scan_count(i, softplus, back=False):
     raw = i["delta"].double() + (i["delta_bias"].double()[:, None] if i.get("delta_bias") is not None else 0)
     dt = R.softplus(raw) if softplus else raw
     worst = float(dt.nan_to_num(0).abs().max() * i["A"].abs().max()) if T else 0.0
-    count = T * (5 * worst + 5) + 3 + N + 64
+    count = T * (20 * worst + 5) + 3 + N + 64
     return count * 2 + D + Bn * T if back else count
 
 
