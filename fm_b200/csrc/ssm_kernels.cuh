@@ -60,24 +60,12 @@ __device__ __forceinline__ float ex2(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + ex2(-kLog2e * v)); }
-
-// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) in (0, 1].  log1p(e) = 2 artanh(r) with
-// r = e / (2 + e) <= 1/3, by its power series 2 (r + r^3/3 + r^5/5 + ...): the first term left out, at
-// r^17, is below 2^-26 of the sum, and small e keep their relative precision.  sigmoid_f is its derivative.
-__device__ __forceinline__ float softplus_f(float v) {
-    const float e = ex2(-kLog2e * fabsf(v));
-    const float r = __fdividef(e, 2.f + e), q = r * r;
-    float s = 1.f / 15.f;
-    s = fmaf(s, q, 1.f / 13.f);
-    s = fmaf(s, q, 1.f / 11.f);
-    s = fmaf(s, q, 1.f / 9.f);
-    s = fmaf(s, q, 1.f / 7.f);
-    s = fmaf(s, q, 1.f / 5.f);
-    s = fmaf(s, q, 1.f / 3.f);
-    s = fmaf(s * q, r, r);
-    return v != v ? v : fmaf(2.f, s, fmaxf(v, 0.f));
+__device__ __forceinline__ float rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp(1.f + ex2(-kLog2e * v)); }
 
 // two fp32 values in one 64-bit register pair; one instruction works on both
 using f2 = unsigned long long;
@@ -102,6 +90,19 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
     f2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) in (0, 1].  log1p(e) = 2 artanh(r) with
+// r = e / (2 + e) <= 1/3, so small e keep their relative precision; artanh(r) / r is a polynomial of degree
+// 4 in r^2, fitted at Chebyshev points of [0, 1/9] and off by at most 8e-9.  sigmoid_f is its derivative.
+__device__ __forceinline__ float softplus_f(float v) {
+    const float e = ex2(-kLog2e * fabsf(v));
+    const float r = e * rcp(2.f + e), q = r * r;
+    float s = fmaf(0.14087329f, q, 0.13980709f);
+    s = fmaf(s, q, 0.20012427f);
+    s = fmaf(s, q, 0.33333158f);
+    s = fmaf(s, q, 1.f);
+    return fmaf(r + r, s, v > 0.f ? v : v != v ? v : 0.f);
 }
 
 template <typename S>
@@ -137,35 +138,50 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes)
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Thread `i` of `n` copies its granules of `rows` rows; src(row) gives a row's first position (t = 0), or
-// null for a row of zeros.  `any`: some valid address, named by the copies that read nothing.
+// Thread `i` of `n` (a multiple of 32) copies its granules of `rows` rows; src(row) gives a row's first
+// position (t = 0), or null for a row of zeros.  `any`: some valid address, named by copies that read nothing.
 template <typename S, bool ALIGNED, typename Src>
 __device__ __forceinline__ void stage_rows(unsigned char *to, int rows, int t0, int lim, int i, int n, const void *any,
                                            Src src) {
     constexpr int G = kSsmTile * static_cast<int>(sizeof(S)) / 16 + (ALIGNED ? 0 : 1);
     const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-    const int step_row = n / G, step_g = n - step_row * G;
-    int row = i / G, g = i - row * G;
-    while (row < rows) {
+    for (int k = i; k < rows * G; k += n) {
+        const int row = k / G, g = k - row * G;  // G is a constant: a shift where the rows are aligned
         const S *first = src(row);
-        int left = 0;
-        const unsigned char *from = nullptr;
-        if (first) {
-            from = reinterpret_cast<const unsigned char *>(first + t0);
-            const unsigned char *end = reinterpret_cast<const unsigned char *>(first + lim);
-            if (!ALIGNED) from -= reinterpret_cast<uintptr_t>(from) & 15;
-            from += g * 16;
-            const int64_t d = end - from;
-            left = d < 0 ? 0 : d > 16 ? 16 : static_cast<int>(d);
-        }
-        copy16(base + row * row_bytes<S>() + g * 16, left ? static_cast<const void *>(from) : any, left);
-        row += step_row;
-        g += step_g;
-        if (g >= G) {
-            g -= G;
-            ++row;
+        const uint32_t dst = base + row * row_bytes<S>() + g * 16;
+        const unsigned char *from = reinterpret_cast<const unsigned char *>(first + t0);
+        if (!ALIGNED) from -= reinterpret_cast<uintptr_t>(from) & 15;
+        from += g * 16;
+        if (first && t0 + kSsmTile + 16 / static_cast<int>(sizeof(S)) <= lim) {  // wholly inside the row
+            copy16(dst, from, 16);
+        } else {
+            const int64_t d = first ? reinterpret_cast<const unsigned char *>(first + lim) - from : 0;
+            const int left = d < 0 ? 0 : d > 16 ? 16 : static_cast<int>(d);
+            copy16(dst, left ? static_cast<const void *>(from) : any, left);
         }
     }
+}
+
+// The same where every granule is whole and aligned: lane `i` of `n` keeps one granule of every n / G-th row,
+// so its addresses advance by constants.  `from`: its granule of row i / G at t = 0.
+template <typename S>
+constexpr int granules = kSsmTile * static_cast<int>(sizeof(S)) / 16;
+template <typename S>
+__device__ __forceinline__ void stage_whole(uint32_t dst, const S *from, int64_t stride, int rows, int i, int n) {
+    const int step = n / granules<S>;
+    for (int r = i / granules<S>; r < rows; r += step) {
+        copy16(dst, from, 16);
+        dst += step * row_bytes<S>();
+        from += step * stride;
+    }
+}
+template <typename S>
+__device__ __forceinline__ uint32_t whole_dst(const void *to, int i) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(to)) + i / granules<S> * row_bytes<S>() + i % granules<S> * 16;
+}
+template <typename S>
+__device__ __forceinline__ const S *whole_src(const S *row, int64_t stride, int i) {
+    return row + i / granules<S> * stride + i % granules<S> * (16 / static_cast<int>(sizeof(S)));
 }
 
 // Element offset of a staged row's first position inside its first granule.
@@ -174,15 +190,20 @@ __device__ __forceinline__ int row_shift(const S *first) {
     return ALIGNED ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / sizeof(S));
 }
 
-// positions 2l, 2l + 1 of a staged row
+// positions 4g ... 4g + 3 of a staged row
 template <typename S, bool ALIGNED>
-__device__ __forceinline__ float2 row_pair(const unsigned char *row, int shift, int l) {
-    const S *p = reinterpret_cast<const S *>(row) + shift + 2 * l;
-    if constexpr (ALIGNED) {
-        if constexpr (sizeof(S) == 4) return *reinterpret_cast<const float2 *>(p);
-        else return unpack2<S>(*reinterpret_cast<const uint32_t *>(p));
+__device__ __forceinline__ void row_four(const unsigned char *row, int shift, int g, float (&f)[4]) {
+    const S *p = reinterpret_cast<const S *>(row) + shift + 4 * g;
+    if constexpr (!ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = Store<S>::to_float(p[i]);
+    } else if constexpr (sizeof(S) == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
     } else {
-        return make_float2(Store<S>::to_float(p[0]), Store<S>::to_float(p[1]));
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        const float2 a = unpack2<S>(v.x), b = unpack2<S>(v.y);
+        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
     }
 }
 
@@ -223,12 +244,32 @@ __device__ __forceinline__ void row_eight(const unsigned char *row, int shift, i
 }
 
 // A tile's 64 floats in shared memory: time lane s keeps positions 8s ... 8s+3 at [4s] and the other
-// four at [32 + 4s], so that 8 time lanes read or write 128 contiguous bytes.  pair_at: positions 2l, 2l + 1.
-__device__ __forceinline__ int pair_at(int l) { return (l & 2) * 16 + (l >> 2) * 4 + (l & 1) * 2; }
+// four at [32 + 4s], so that 8 time lanes read or write 128 contiguous bytes.
+__device__ __forceinline__ float4 &tile_four(float *base, int g) {  // positions 4g ... 4g + 3
+    return *reinterpret_cast<float4 *>(base + (g & 1) * 32 + (g >> 1) * 4);
+}
+__device__ __forceinline__ void tile_put(float *base, int g, const float (&f)[4]) { tile_four(base, g) = make_float4(f[0], f[1], f[2], f[3]); }
+__device__ __forceinline__ void tile_take(float *base, int g, float (&f)[4]) {
+    const float4 v = tile_four(base, g);
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+}
 __device__ __forceinline__ void tile_get(const float *base, int s, f2 (&f)[4]) {
     const float4 p = *reinterpret_cast<const float4 *>(base + 4 * s);
     const float4 q = *reinterpret_cast<const float4 *>(base + 32 + 4 * s);
     f[0] = pk(p.x, p.y), f[1] = pk(p.z, p.w), f[2] = pk(q.x, q.y), f[3] = pk(q.z, q.w);
+}
+
+// the same, every value twice in a pair
+__device__ __forceinline__ void tile_get_twice(const float *base, int s, f2 (&f)[8]) {
+    const float4 p = *reinterpret_cast<const float4 *>(base + 4 * s);
+    const float4 q = *reinterpret_cast<const float4 *>(base + 32 + 4 * s);
+    f[0] = pk(p.x, p.x), f[1] = pk(p.y, p.y), f[2] = pk(p.z, p.z), f[3] = pk(p.w, p.w);
+    f[4] = pk(q.x, q.x), f[5] = pk(q.y, q.y), f[6] = pk(q.z, q.z), f[7] = pk(q.w, q.w);
+}
+// two rows of 8 positions as 8 pairs (first row, second row)
+__device__ __forceinline__ void zip8(const f2 (&a)[4], const f2 (&b)[4], f2 (&o)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[2 * k] = pk(lo(a[k]), lo(b[k])), o[2 * k + 1] = pk(hi(a[k]), hi(b[k]));
 }
 
 // Sum of v over the 4 state lanes, spread so that each of them keeps two positions: state lane q gets
@@ -272,6 +313,29 @@ __device__ __forceinline__ float lane_scan(float P, float &S, float carry, int s
     const float in = UP ? __shfl_up_sync(kFullMask, S, 1, 8) : __shfl_down_sync(kFullMask, S, 1, 8);
     return r == 0 ? carry : in;
 }
+// The same for two states at once, packed.
+template <bool UP>
+__device__ __forceinline__ f2 lane_move(f2 v, int k) {
+    return UP ? pk(__shfl_up_sync(kFullMask, lo(v), k, 8), __shfl_up_sync(kFullMask, hi(v), k, 8))
+              : pk(__shfl_down_sync(kFullMask, lo(v), k, 8), __shfl_down_sync(kFullMask, hi(v), k, 8));
+}
+template <bool UP>
+__device__ __forceinline__ f2 lane_scan2(f2 P, f2 &S, f2 carry, int s) {
+    const int r = UP ? s : 7 - s;
+    if (r == 0) S = fma2(P, carry, S);
+#pragma unroll
+    for (int k = 1; k < 8; k *= 2) {
+        const f2 Sp = lane_move<UP>(S, k);
+        f2 Pp = 0;
+        if (k < 4) Pp = lane_move<UP>(P, k);
+        if (r >= k) {
+            S = fma2(P, Sp, S);
+            if (k < 4) P = mul2(P, Pp);
+        }
+    }
+    const f2 in = lane_move<UP>(S, 1);
+    return r == 0 ? carry : in;
+}
 __device__ __forceinline__ float product8(const f2 (&a)[4]) {
     const f2 m = mul2(mul2(a[0], a[1]), mul2(a[2], a[3]));
     return lo(m) * hi(m);
@@ -302,30 +366,55 @@ __device__ __forceinline__ int ssm_length(const SsmProblem<S> &p, int64_t b) {
     return static_cast<int>(n < 0 ? 0 : n > p.T ? p.T : n);
 }
 
-// Time step of a raw value; a position behind the sequence gets 0, which makes it the identity step.
-__device__ __forceinline__ float time_step(float raw, float bias, int softplus, bool live) {
-    const float r = raw + bias;
-    return live ? (softplus ? softplus_f(r) : r) : 0.f;
+// Zeros at the positions of t ... t + 3 that are not below `len`.
+__device__ __forceinline__ void cut_four(float (&f)[4], int t, int len) {
+    if (t + 4 > len) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t + i >= len) f[i] = 0.f;
+    }
 }
 
-// Positions t, t + 1 of an output row, those below T only.
+// Time steps of four raw values; positions behind the sequence get 0, which makes them identity steps.
+__device__ __forceinline__ void time_steps(float (&f)[4], float bias, int softplus, int t, int len) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] += bias;
+        if (softplus) f[i] = softplus_f(f[i]);
+    }
+    cut_four(f, t, len);
+}
+
+// Positions t ... t + 3 of an output row, those below T only.
 template <typename S, bool ALIGNED>
-__device__ __forceinline__ void store_pair(S *__restrict__ row, int t, int T, float a, float b) {
-    if (ALIGNED && t + 2 <= T) {
+__device__ __forceinline__ void store_four(S *__restrict__ row, int t, int T, const float (&f)[4]) {
+    if (ALIGNED && t + 4 <= T) {
         if constexpr (sizeof(S) == 4) {
-            *reinterpret_cast<float2 *>(row + t) = make_float2(a, b);
+            *reinterpret_cast<float4 *>(row + t) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
             union {
-                S h[2];
-                uint32_t w;
+                S h[4];
+                uint2 w;
             } v;
-            v.h[0] = from_float<S>(a);
-            v.h[1] = from_float<S>(b);
-            *reinterpret_cast<uint32_t *>(row + t) = v.w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v.h[i] = from_float<S>(f[i]);
+            *reinterpret_cast<uint2 *>(row + t) = v.w;
         }
     } else {
-        if (t < T) row[t] = from_float<S>(a);
-        if (t + 1 < T) row[t + 1] = from_float<S>(b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t + i < T) row[t + i] = from_float<S>(f[i]);
+    }
+}
+
+// `count` floats, copied by the lanes of a warp between rows of NP floats in shared memory and rows of N in
+// global memory (N == NP: one run of whole vectors).
+__device__ __forceinline__ void states_out(float *__restrict__ to, const float *from, int rows, int N, int NP, int lane) {
+    if (N == NP && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+        for (int i = lane; i < rows * N / 4; i += 32) reinterpret_cast<float4 *>(to)[i] = reinterpret_cast<const float4 *>(from)[i];
+    } else {
+        for (int c = 0; c < rows; ++c)
+            for (int n = lane; n < N; n += 32) to[static_cast<int64_t>(c) * N + n] = from[c * NP + n];
     }
 }
 
@@ -334,15 +423,15 @@ template <typename S>
 inline __host__ __device__ size_t ssm_bc_bytes() { return 2 * 2 * kSsmNB * row_bytes<S>(); }
 template <typename S>
 inline __host__ __device__ size_t ssm_fwd_warp_bytes(int cw, int NP) {
-    return cw * (2 * 3 * row_bytes<S>() + sizeof(float) * (3 * kSsmTile + 2 * NP));
+    return cw * (2 * 3 * row_bytes<S>() + sizeof(float) * (3 * kSsmTile + 2 * NP + 4));
 }
 template <typename S>
 inline __host__ __device__ size_t ssm_bwd_warp_bytes(int cw, int NP) {
-    return cw * (2 * 4 * row_bytes<S>() + sizeof(float) * (6 * kSsmTile + 4 * NP + 4));
+    return cw * (2 * 4 * row_bytes<S>() + sizeof(float) * (6 * kSsmTile + 4 * NP + 36));
 }
 
 template <typename S, bool ALIGNED>
-__global__ void __launch_bounds__(kSsmFwdWarps * 32)
+__global__ void __launch_bounds__(kSsmFwdWarps * 32, 3)
 ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict__ h_last,
                    float *__restrict__ checkpoints) {
     extern __shared__ __align__(16) unsigned char ssm_smem[];
@@ -352,7 +441,7 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
     unsigned char *raw = ssm_smem + ssm_bc_bytes<S>() + (threadIdx.x >> 5) * ssm_fwd_warp_bytes<S>(p.cw, p.NP);
     float *dt_ = reinterpret_cast<float *>(raw + 2 * 3 * p.cw * RB);
     float *u_ = dt_ + p.cw * kSsmTile, *y_ = u_ + p.cw * kSsmTile;
-    float *h_ = y_ + p.cw * kSsmTile, *A_ = h_ + p.cw * p.NP;
+    float *h_ = y_ + p.cw * kSsmTile, *A_ = h_ + p.cw * p.NP, *bias_ = A_ + p.cw * p.NP, *D_ = bias_ + p.cw;
     const int len = ssm_length(p, w.b);
     const int64_t row0 = w.b * p.channels + w.d0;
     const S *xrow = p.x + w.b * p.xs[0] + w.d0 * p.xs[1], *drow = p.delta + w.b * p.ds[0] + w.d0 * p.ds[1];
@@ -364,28 +453,47 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
             A_[c * p.NP + n] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
             h_[c * p.NP + n] = n < p.N && p.h0 ? p.h0[(row0 + c) * p.N + n] : 0.f;
         }
+    if (lane < w.nc) {  // at most 8 channels
+        bias_[lane] = p.bias ? p.bias[w.d0 + lane] : 0.f;
+        D_[lane] = p.D ? p.D[w.d0 + lane] : 0.f;
+    }
 
     const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
-    const int kinds = p.z ? 3 : 2;
     const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
+    const S *xw = whole_src(xrow, p.xs[1], lane), *dw = whole_src(drow, p.ds[1], lane);
+    const S *zw = p.z ? whole_src(zrow, p.zs[1], lane) : nullptr;
+    const S *Bw = whole_src(Brow, p.Bs[2], threadIdx.x), *Cw = whole_src(Crow, p.Cs[2], threadIdx.x);
     auto stage = [&](int tile, int nb, int step) {
         const int t0 = tile * kSsmTile;
-        stage_rows<S, ALIGNED>(ssm_smem + (step & 1) * (2 * kSsmNB * RB), 2 * kSsmNB, t0, len, threadIdx.x,
-                               kSsmFwdWarps * 32, any, [&](int r) -> const S * {
-                                   const int n = nb * kSsmNB + (r & (kSsmNB - 1));
-                                   return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
-                               });
-        if (nb == 0)
-            stage_rows<S, ALIGNED>(raw + (tile & 1) * (3 * p.cw * RB), w.nc * kinds, t0, len, lane, 32, any, [&](int r) -> const S * {
-                const int kind = r / w.nc, c = r - kind * w.nc;  // rows: x of every channel, then delta, then z
-                return kind == 0 ? xrow + c * p.xs[1] : kind == 1 ? drow + c * p.ds[1] : zrow + c * p.zs[1];
+        unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB), *to = raw + (tile & 1) * (3 * p.cw * RB);
+        if (ALIGNED && t0 + kSsmTile <= len) {
+            constexpr int n = kSsmFwdWarps * 32;
+            if ((nb + 1) * kSsmNB <= p.N) {
+                stage_whole<S>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
+            }
+            if (nb == 0) {
+                stage_whole<S>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
+                stage_whole<S>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
+                if (p.z) stage_whole<S>(whole_dst<S>(to + 2 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
+            }
+        } else if (nb == 0) {
+            stage_rows<S, ALIGNED>(to, w.nc, t0, len, lane, 32, any, [&](int c) { return xrow + c * p.xs[1]; });
+            stage_rows<S, ALIGNED>(to + p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return drow + c * p.ds[1]; });
+            if (p.z)
+                stage_rows<S, ALIGNED>(to + 2 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return zrow + c * p.zs[1]; });
+        }
+        if (!ALIGNED || t0 + kSsmTile > len || (nb + 1) * kSsmNB > p.N)
+            stage_rows<S, ALIGNED>(bc, 2 * kSsmNB, t0, len, threadIdx.x, kSsmFwdWarps * 32, any, [&](int r) -> const S * {
+                const int n = nb * kSsmNB + (r & (kSsmNB - 1));
+                return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
             });
         copies_commit();
     };
     if (live_tiles > 0) stage(0, 0, 0);
 
     for (int tile = 0, step = 0; tile < live_tiles; ++tile) {
-        const int t = tile * kSsmTile + 2 * lane;  // this lane's two positions outside the state loop
+        const int g = lane & 15, t = tile * kSsmTile + 4 * g;  // outside the state loop a lane has four positions of a channel
         const unsigned char *mine = raw + (tile & 1) * (3 * p.cw * RB);
         for (int nb = 0; nb < blocks; ++nb, ++step) {
             copies_wait();
@@ -393,95 +501,100 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
             if (nb + 1 < blocks) stage(tile, nb + 1, step + 1);
             else if (tile + 1 < live_tiles) stage(tile + 1, 0, step + 1);
             if (nb == 0) {
-                for (int c = 0; c < w.nc; ++c) {
-                    const float bias = p.bias ? p.bias[w.d0 + c] : 0.f;
-                    const float2 x = row_pair<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), lane);
-                    const float2 r = row_pair<S, ALIGNED>(mine + (w.nc + c) * RB, row_shift<S, ALIGNED>(drow + c * p.ds[1]), lane);
-                    const float2 dt = make_float2(time_step(r.x, bias, p.softplus, t < len),
-                                                  time_step(r.y, bias, p.softplus, t + 1 < len));
-                    *reinterpret_cast<float2 *>(dt_ + c * kSsmTile + pair_at(lane)) = dt;
-                    *reinterpret_cast<float2 *>(u_ + c * kSsmTile + pair_at(lane)) = make_float2(dt.x * x.x, dt.y * x.y);
+                for (int c = lane >> 4; c < w.nc; c += 2) {
+                    float x[4], dt[4];
+                    row_four<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), g, x);
+                    row_four<S, ALIGNED>(mine + (p.cw + c) * RB, row_shift<S, ALIGNED>(drow + c * p.ds[1]), g, dt);
+                    time_steps(dt, bias_[c], p.softplus, t, len);
+                    tile_put(dt_ + c * kSsmTile, g, dt);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] *= dt[i];
+                    tile_put(u_ + c * kSsmTile, g, x);
                 }
-                if (checkpoints) {
-                    float *ck = checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
-                    for (int c = 0; c < w.nc; ++c)
-                        for (int n = lane; n < p.N; n += 32) ck[c * p.N + n] = h_[c * p.NP + n];
-                }
+                if (checkpoints)
+                    states_out(checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N, h_, w.nc, p.N, p.NP, lane);
                 __syncwarp();
             }
             const int n0 = nb * kSsmNB + q * kSsmNL;
-            f2 B[kSsmNL][4], C[kSsmNL][4];
+            f2 B[2][8], C[2][8];  // [pair of states][position]
             {
                 const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
 #pragma unroll
-                for (int j = 0; j < kSsmNL; ++j) {
-                    const int r = q * kSsmNL + j;
-                    row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(Brow + (n0 + j) * p.Bs[2]), s, B[j]);
-                    row_eight<S, ALIGNED>(bc + (kSsmNB + r) * RB, row_shift<S, ALIGNED>(Crow + (n0 + j) * p.Cs[2]), s, C[j]);
+                for (int j = 0; j < 2; ++j) {
+                    const int r = q * kSsmNL + 2 * j, n = n0 + 2 * j;
+                    f2 e[4], o[4];
+                    row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(Brow + n * p.Bs[2]), s, e);
+                    row_eight<S, ALIGNED>(bc + (r + 1) * RB, row_shift<S, ALIGNED>(Brow + (n + 1) * p.Bs[2]), s, o);
+                    zip8(e, o, B[j]);
+                    row_eight<S, ALIGNED>(bc + (kSsmNB + r) * RB, row_shift<S, ALIGNED>(Crow + n * p.Cs[2]), s, e);
+                    row_eight<S, ALIGNED>(bc + (kSsmNB + r + 1) * RB, row_shift<S, ALIGNED>(Crow + (n + 1) * p.Cs[2]), s, o);
+                    zip8(e, o, C[j]);
                 }
             }
             for (int c = 0; c < w.nc; ++c) {
-                f2 dt[4], u[4], y[4];
-                tile_get(dt_ + c * kSsmTile, s, dt);
-                tile_get(u_ + c * kSsmTile, s, u);
+                f2 dt[8], u[8], y[8];
+                tile_get_twice(dt_ + c * kSsmTile, s, dt);
+                tile_get_twice(u_ + c * kSsmTile, s, u);
                 const float4 A4 = *reinterpret_cast<const float4 *>(A_ + c * p.NP + n0);
-                float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
+                const float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
                 __syncwarp();  // the carries are read before the last time lane replaces them
-                const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
-                float hv[4] = {h4.x, h4.y, h4.z, h4.w};
+                const f2 Av[2] = {pk(A4.x, A4.y), pk(A4.z, A4.w)};
+                f2 hv[2] = {pk(h4.x, h4.y), pk(h4.z, h4.w)};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = 0;
+                for (int j = 0; j < 2; ++j) {
+                    f2 a[8], b[8];
 #pragma unroll
-                for (int j = 0; j < kSsmNL; ++j) {
-                    const f2 Ad = pk(Av[j], Av[j]);
-                    f2 a[4], b[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const f2 e = mul2(dt[k], Ad);
-                        a[k] = pk(ex2(lo(e)), ex2(hi(e)));
-                        b[k] = mul2(u[k], B[j][k]);
+                    for (int i = 0; i < 8; ++i) {
+                        const f2 e = mul2(dt[i], Av[j]);
+                        a[i] = pk(ex2(lo(e)), ex2(hi(e)));
+                        b[i] = mul2(u[i], B[j][i]);
                     }
-                    float S0 = lo(b[0]);
+                    f2 S0 = b[0], P = a[0];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k) S0 = fmaf(lo(a[k]), S0, lo(b[k]));
-                        S0 = fmaf(hi(a[k]), S0, hi(b[k]));
+                    for (int i = 1; i < 8; ++i) {
+                        S0 = fma2(a[i], S0, b[i]);
+                        P = mul2(P, a[i]);
                     }
-                    float h = lane_scan<true>(product8(a), S0, hv[j], s);
+                    f2 h = lane_scan2<true>(P, S0, hv[j], s);
                     hv[j] = S0;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float h1 = fmaf(lo(a[k]), h, lo(b[k]));
-                        h = fmaf(hi(a[k]), h1, hi(b[k]));
-                        y[k] = fma2(C[j][k], pk(h1, h), y[k]);
+                    for (int i = 0; i < 8; ++i) {
+                        h = fma2(a[i], h, b[i]);
+                        y[i] = j ? fma2(C[j][i], h, y[i]) : mul2(C[j][i], h);
                     }
                 }
-                if (s == 7) *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(hv[0], hv[1], hv[2], hv[3]);
-                tile_sum(y_ + c * kSsmTile, s, q, y, nb == 0);
+                if (s == 7)
+                    *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(lo(hv[0]), hi(hv[0]), lo(hv[1]), hi(hv[1]));
+                f2 sum[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] = pk(lo(y[2 * k]) + hi(y[2 * k]), lo(y[2 * k + 1]) + hi(y[2 * k + 1]));
+                tile_sum(y_ + c * kSsmTile, s, q, sum, nb == 0);
             }
         }
         __syncwarp();
-        for (int c = 0; c < w.nc; ++c) {
-            float2 y = *reinterpret_cast<const float2 *>(y_ + c * kSsmTile + pair_at(lane));
+        for (int c = lane >> 4; c < w.nc; c += 2) {
+            float y[4], v[4];
+            tile_take(y_ + c * kSsmTile, g, y);
             if (p.D) {
-                const float D = p.D[w.d0 + c];
-                const float2 x = row_pair<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), lane);
-                y = make_float2(fmaf(D, x.x, y.x), fmaf(D, x.y, y.y));
+                row_four<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(xrow + c * p.xs[1]), g, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = fmaf(D_[c], v[i], y[i]);
             }
             if (p.z) {
-                const float2 z = row_pair<S, ALIGNED>(mine + (2 * w.nc + c) * RB, row_shift<S, ALIGNED>(zrow + c * p.zs[1]), lane);
-                y = make_float2(y.x * z.x * sigmoid_f(z.x), y.y * z.y * sigmoid_f(z.y));
+                row_four<S, ALIGNED>(mine + (2 * p.cw + c) * RB, row_shift<S, ALIGNED>(zrow + c * p.zs[1]), g, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] *= v[i] * sigmoid_f(v[i]);
             }
-            store_pair<S, ALIGNED>(out + (row0 + c) * p.T, t, p.T, t < len ? y.x : 0.f, t + 1 < len ? y.y : 0.f);
+            cut_four(y, t, len);
+            store_four<S, ALIGNED>(out + (row0 + c) * p.T, t, p.T, y);
         }
     }
     __syncwarp();
+    const float zero[4] = {};
     for (int tile = live_tiles; tile < p.tiles; ++tile)  // behind the sequence: zeros
-        for (int c = 0; c < w.nc; ++c)
-            store_pair<S, ALIGNED>(out + (row0 + c) * p.T, tile * kSsmTile + 2 * lane, p.T, 0.f, 0.f);
-    if (h_last)
-        for (int c = 0; c < w.nc; ++c)
-            for (int n = lane; n < p.N; n += 32) h_last[(row0 + c) * p.N + n] = h_[c * p.NP + n];
+        for (int c = lane >> 4; c < w.nc; c += 2)
+            store_four<S, ALIGNED>(out + (row0 + c) * p.T, tile * kSsmTile + 4 * (lane & 15), p.T, zero);
+    if (h_last && w.nc > 0) states_out(h_last + row0 * p.N, h_, w.nc, p.N, p.NP, lane);
 }
 
 // What the backward writes; the partial sums live in the caller's workspace.
@@ -510,7 +623,7 @@ template <typename S, bool ALIGNED, bool GATED>
 __global__ void __launch_bounds__(kSsmBwdWarps * 32, 1)
 ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
     extern __shared__ __align__(16) unsigned char ssm_smem[];
-    constexpr int W = kSsmBwdWarps, RB = row_bytes<S>(), kinds = GATED ? 4 : 3;
+    constexpr int W = kSsmBwdWarps, RB = row_bytes<S>();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3;
     const SsmPlace w = ssm_place(p, W);
     float *red = reinterpret_cast<float *>(ssm_smem + ssm_bc_bytes<S>());  // [warp][64][lane]
@@ -518,7 +631,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
     const int ct = p.cw * kSsmTile, cn = p.cw * p.NP;
     float *dt_ = reinterpret_cast<float *>(raw + 2 * 4 * p.cw * RB);
     float *u_ = dt_ + ct, *dy_ = u_ + ct, *gB_ = dy_ + ct, *q_ = gB_ + ct, *y_ = q_ + ct;
-    float *A_ = y_ + ct, *h_ = A_ + cn, *c_ = h_ + cn, *dA_ = c_ + cn, *dD_ = dA_ + cn, *db_ = dD_ + p.cw;
+    float *A_ = y_ + ct, *h_ = A_ + cn, *c_ = h_ + cn, *dA_ = c_ + cn, *dD_ = dA_ + cn, *bias_ = dD_ + 32 * p.cw, *D_ = bias_ + p.cw;
     const int len = ssm_length(p, w.b);
     const int64_t row0 = w.b * p.channels + w.d0;
     const int Tpad = p.tiles * kSsmTile;
@@ -535,42 +648,64 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             h_[i] = 0.f;
             dA_[i] = 0.f;
         }
-        if (lane == 0) dD_[c] = db_[c] = 0.f;
+        dD_[c * 32 + lane] = 0.f;
+        if (lane == 0) {
+            bias_[c] = p.bias ? p.bias[w.d0 + c] : 0.f;
+            D_[c] = p.D ? p.D[w.d0 + c] : 0.f;
+        }
     }
 
     const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
     const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
+    const int64_t T = p.T;
+    const S *xw = whole_src(xrow, p.xs[1], lane), *dw = whole_src(drow, p.ds[1], lane), *gw = whole_src(grow, T, lane);
+    const S *zw = GATED ? whole_src(zrow, p.zs[1], lane) : nullptr;
+    const S *Bw = whole_src(Brow, p.Bs[2], threadIdx.x), *Cw = whole_src(Crow, p.Cs[2], threadIdx.x);
     auto stage = [&](int tile, int nb, int step) {
         const int t0 = tile * kSsmTile;
-        stage_rows<S, ALIGNED>(ssm_smem + (step & 1) * (2 * kSsmNB * RB), 2 * kSsmNB, t0, len, threadIdx.x, W * 32, any,
-                               [&](int r) -> const S * {
-                                   const int n = nb * kSsmNB + (r & (kSsmNB - 1));
-                                   return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
-                               });
-        if (nb == 0)
-            stage_rows<S, ALIGNED>(raw + (tile & 1) * (4 * p.cw * RB), w.nc * kinds, t0, len, lane, 32, any, [&](int r) -> const S * {
-                const int kind = r / w.nc, c = r - kind * w.nc;  // rows: x of every channel, then delta, grad_out, z
-                return kind == 0   ? xrow + c * p.xs[1]
-                       : kind == 1 ? drow + c * p.ds[1]
-                       : kind == 2 ? grow + static_cast<int64_t>(c) * p.T
-                                   : zrow + c * p.zs[1];
+        unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB), *to = raw + (tile & 1) * (4 * p.cw * RB);
+        if (ALIGNED && t0 + kSsmTile <= len) {
+            constexpr int n = W * 32;
+            if ((nb + 1) * kSsmNB <= p.N) {
+                stage_whole<S>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
+            }
+            if (nb == 0) {
+                stage_whole<S>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
+                stage_whole<S>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
+                stage_whole<S>(whole_dst<S>(to + 2 * p.cw * RB, lane), gw + t0, T, w.nc, lane, 32);
+                if (GATED) stage_whole<S>(whole_dst<S>(to + 3 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
+            }
+        } else if (nb == 0) {
+            stage_rows<S, ALIGNED>(to, w.nc, t0, len, lane, 32, any, [&](int c) { return xrow + c * p.xs[1]; });
+            stage_rows<S, ALIGNED>(to + p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return drow + c * p.ds[1]; });
+            stage_rows<S, ALIGNED>(to + 2 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return grow + c * T; });
+            if (GATED)
+                stage_rows<S, ALIGNED>(to + 3 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return zrow + c * p.zs[1]; });
+        }
+        if (!ALIGNED || t0 + kSsmTile > len || (nb + 1) * kSsmNB > p.N)
+            stage_rows<S, ALIGNED>(bc, 2 * kSsmNB, t0, len, threadIdx.x, W * 32, any, [&](int r) -> const S * {
+                const int n = nb * kSsmNB + (r & (kSsmNB - 1));
+                return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
             });
         copies_commit();
     };
-    auto row_at = [&](const unsigned char *mine, int kind, int c) {
+    const int g4 = lane & 15;  // outside the state loop a lane has four positions of a channel
+    auto row_at = [&](const unsigned char *mine, int kind, int c, float (&f)[4]) {
         const S *first = kind == 0   ? xrow + c * p.xs[1]
                          : kind == 1 ? drow + c * p.ds[1]
-                         : kind == 2 ? grow + static_cast<int64_t>(c) * p.T
+                         : kind == 2 ? grow + c * T
                                      : zrow + c * p.zs[1];
-        return row_pair<S, ALIGNED>(mine + (kind * w.nc + c) * RB, row_shift<S, ALIGNED>(first), lane);
+        row_four<S, ALIGNED>(mine + (kind * p.cw + c) * RB, row_shift<S, ALIGNED>(first), g4, f);
     };
 
     for (int tile = p.tiles - 1; tile >= live_tiles; --tile) {  // behind the sequence: zeros
-        const int t = tile * kSsmTile + 2 * lane;
-        for (int c = 0; c < w.nc; ++c) {
-            store_pair<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
-            store_pair<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
-            if (GATED) store_pair<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T, 0.f, 0.f);
+        const int t = tile * kSsmTile + 4 * g4;
+        const float zero[4] = {};
+        for (int c = lane >> 4; c < w.nc; c += 2) {
+            store_four<S, ALIGNED>(o.dx + (row0 + c) * T, t, p.T, zero);
+            store_four<S, ALIGNED>(o.ddelta + (row0 + c) * T, t, p.T, zero);
+            if (GATED) store_four<S, ALIGNED>(o.dz + (row0 + c) * T, t, p.T, zero);
         }
         for (int i = threadIdx.x; i < 2 * p.N * kSsmTile; i += W * 32)
             bc_out[static_cast<int64_t>(i / kSsmTile) * Tpad + tile * kSsmTile + i % kSsmTile] = 0.f;
@@ -578,7 +713,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
     if (live_tiles > 0) stage(live_tiles - 1, 0, 0);
 
     for (int tile = live_tiles - 1, step = 0; tile >= 0; --tile) {
-        const int t = tile * kSsmTile + 2 * lane;
+        const int t = tile * kSsmTile + 4 * g4;
         const unsigned char *mine = raw + (tile & 1) * (4 * p.cw * RB);
         for (int nb = 0; nb < blocks; ++nb, ++step) {
             copies_wait();
@@ -587,21 +722,25 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             else if (tile > 0) stage(tile - 1, 0, step + 1);
             if (nb == 0) {
                 const float *ck = o.checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
-                for (int c = 0; c < w.nc; ++c) {
+                for (int c = 0; c < w.nc; ++c)
                     for (int n = lane; n < p.N; n += 32) h_[c * p.NP + n] = ck[c * p.N + n];
-                    const float bias = p.bias ? p.bias[w.d0 + c] : 0.f;
-                    const float2 x = row_at(mine, 0, c), r = row_at(mine, 1, c);
-                    float2 dy = row_at(mine, 2, c);
+                for (int c = lane >> 4; c < w.nc; c += 2) {
+                    float x[4], dt[4], dy[4];
+                    row_at(mine, 0, c, x);
+                    row_at(mine, 1, c, dt);
+                    row_at(mine, 2, c, dy);
                     if (GATED) {
-                        const float2 z = row_at(mine, 3, c);
-                        dy = make_float2(dy.x * z.x * sigmoid_f(z.x), dy.y * z.y * sigmoid_f(z.y));
+                        float z[4];
+                        row_at(mine, 3, c, z);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dy[i] *= z[i] * sigmoid_f(z[i]);
                     }
-                    const float2 dt = make_float2(time_step(r.x, bias, p.softplus, t < len),
-                                                  time_step(r.y, bias, p.softplus, t + 1 < len));
-                    const int at = c * kSsmTile + pair_at(lane);
-                    *reinterpret_cast<float2 *>(dt_ + at) = dt;
-                    *reinterpret_cast<float2 *>(u_ + at) = make_float2(dt.x * x.x, dt.y * x.y);
-                    *reinterpret_cast<float2 *>(dy_ + at) = dy;
+                    time_steps(dt, bias_[c], p.softplus, t, len);
+                    tile_put(dt_ + c * kSsmTile, g4, dt);
+                    tile_put(dy_ + c * kSsmTile, g4, dy);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] *= dt[i];
+                    tile_put(u_ + c * kSsmTile, g4, x);
                 }
                 __syncwarp();
             }
@@ -726,37 +865,47 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             }
         }
 
-        for (int c = 0; c < w.nc; ++c) {
-            const int at = c * kSsmTile + pair_at(lane);
-            const float2 dt = *reinterpret_cast<const float2 *>(dt_ + at), dy = *reinterpret_cast<const float2 *>(dy_ + at);
-            const float2 gB = *reinterpret_cast<const float2 *>(gB_ + at), Q = *reinterpret_cast<const float2 *>(q_ + at);
-            const float D = p.D ? p.D[w.d0 + c] : 0.f, bias = p.bias ? p.bias[w.d0 + c] : 0.f;
-            const float2 x = row_at(mine, 0, c), r = row_at(mine, 1, c);
-            const bool on0 = t < len, on1 = t + 1 < len;
-            store_pair<S, ALIGNED>(o.dx + (row0 + c) * p.T, t, p.T, on0 ? fmaf(dt.x, gB.x, D * dy.x) : 0.f,
-                                   on1 ? fmaf(dt.y, gB.y, D * dy.y) : 0.f);
-            float2 d = make_float2(fmaf(kLn2, Q.x, x.x * gB.x), fmaf(kLn2, Q.y, x.y * gB.y));
-            if (p.softplus) d = make_float2(d.x * sigmoid_f(r.x + bias), d.y * sigmoid_f(r.y + bias));
-            d = make_float2(on0 ? d.x : 0.f, on1 ? d.y : 0.f);
-            store_pair<S, ALIGNED>(o.ddelta + (row0 + c) * p.T, t, p.T, d.x, d.y);
-            if (GATED) {
-                const float2 y = *reinterpret_cast<const float2 *>(y_ + at);
-                const float2 z = row_at(mine, 3, c), up = row_at(mine, 2, c);
-                const float g0 = sigmoid_f(z.x), g1 = sigmoid_f(z.y);
-                store_pair<S, ALIGNED>(o.dz + (row0 + c) * p.T, t, p.T,
-                                       on0 ? up.x * fmaf(D, x.x, y.x) * g0 * fmaf(z.x, 1.f - g0, 1.f) : 0.f,
-                                       on1 ? up.y * fmaf(D, x.y, y.y) * g1 * fmaf(z.y, 1.f - g1, 1.f) : 0.f);
-            }
-            float sD = fmaf(dy.x, x.x, dy.y * x.y), sb = d.x + d.y;
+        for (int c = lane >> 4; c < w.nc; c += 2) {
+            const int at = c * kSsmTile;
+            float dt[4], dy[4], gB[4], Q[4], x[4], r[4], v[4], sD = 0.f, sb = 0.f;
+            tile_take(dt_ + at, g4, dt);
+            tile_take(dy_ + at, g4, dy);
+            tile_take(gB_ + at, g4, gB);
+            tile_take(q_ + at, g4, Q);
+            row_at(mine, 0, c, x);
+            row_at(mine, 1, c, r);
+            const float D = D_[c], bias = bias_[c];
 #pragma unroll
-            for (int k = 1; k < 32; k *= 2) {
-                sD += __shfl_xor_sync(kFullMask, sD, k);
-                sb += __shfl_xor_sync(kFullMask, sb, k);
+            for (int i = 0; i < 4; ++i) {
+                v[i] = fmaf(dt[i], gB[i], D * dy[i]);
+                sD = fmaf(dy[i], x[i], sD);
             }
-            if (lane == 0) {
-                dD_[c] += sD;
-                db_[c] += sb;
+            cut_four(v, t, len);
+            store_four<S, ALIGNED>(o.dx + (row0 + c) * T, t, p.T, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = fmaf(kLn2, Q[i], x[i] * gB[i]);
+                if (p.softplus) v[i] *= sigmoid_f(r[i] + bias);
             }
+            cut_four(v, t, len);
+            store_four<S, ALIGNED>(o.ddelta + (row0 + c) * T, t, p.T, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sb += v[i];
+            if (GATED) {
+                float z[4], up[4];
+                tile_take(y_ + at, g4, v);
+                row_at(mine, 3, c, z);
+                row_at(mine, 2, c, up);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float sg = sigmoid_f(z[i]);
+                    v[i] = up[i] * fmaf(D, x[i], v[i]) * sg * fmaf(z[i], 1.f - sg, 1.f);
+                }
+                cut_four(v, t, len);
+                store_four<S, ALIGNED>(o.dz + (row0 + c) * T, t, p.T, v);
+            }
+            float2 *sums = reinterpret_cast<float2 *>(dD_) + c * 16 + g4;  // this lane's share of grad D, grad delta_bias
+            *sums = make_float2(sums->x + sD, sums->y + sb);
         }
     }
     __syncwarp();
@@ -766,9 +915,10 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             o.a_part[(row0 + c) * p.N + n] = dA_[k];
             if (o.dh0) o.dh0[(row0 + c) * p.N + n] = c_[k];
         }
-        if (lane == 0) {
-            o.d_part[(w.b * 2) * p.channels + w.d0 + c] = dD_[c];
-            o.d_part[(w.b * 2 + 1) * p.channels + w.d0 + c] = db_[c];
+        if (lane < 2) {  // grad D, grad delta_bias: the 16 lanes' shares in order
+            float v = 0.f;
+            for (int i = 0; i < 16; ++i) v += dD_[(c * 16 + i) * 2 + lane];
+            o.d_part[(w.b * 2 + lane) * p.channels + w.d0 + c] = v;
         }
     }
 }
