@@ -49,7 +49,7 @@ int ssm_check(const fms_ssm_args *a) {
     if (!dtype_ok(a->dtype)) return FMS_ERR_BAD_DTYPE;
     if (a->batch < 0 || a->channels < 0 || a->T < 0 || a->groups < 1 || a->states < 1) return FMS_ERR_BAD_SHAPE;
     if (a->channels % a->groups) return FMS_ERR_BAD_SHAPE;
-    if (a->states > FMS_SSM_MAX_STATES || a->T > 0x7fffffff - 4096) return FMS_ERR_TOO_LARGE;
+    if (a->states > FMS_SSM_MAX_STATES || a->T > 0x7fffffff - 4096 || a->channels > 0x7fffffff) return FMS_ERR_TOO_LARGE;
     if (!product_ok({a->batch, a->channels, std::max<int64_t>(a->T, a->states)}) ||
         !product_ok({a->batch, a->groups, a->states, a->T}) ||
         !product_ok({a->batch, a->channels, a->T / fms::kSsmTile + 1, a->states}))
@@ -212,19 +212,27 @@ int launch_ssm_backward(const fms_ssm_args *a, fms::SsmGrads<S> o, S *dB, S *dC,
     return sum_slices(o.d_part + p.channels, dbias, p.channels, p.batch, 2 * p.channels, st);
 }
 
+template <typename S, bool VEC, int U>
+int launch_ssm_step_u(const fms::SsmProblem<S> &p, float *state, int64_t pool, const int64_t *slots, void *out, int log_L,
+                      cudaStream_t st) {
+    const int per = 128 >> log_L;
+    const dim3 grid(static_cast<unsigned>((p.per_group + per * U - 1) / (per * U)), static_cast<unsigned>(p.groups),
+                    static_cast<unsigned>(std::min<int64_t>(p.batch, 65535)));
+    const bool bc_vec = p.N % 8 == 0 && rows16(p.B, p.Bs, 2, sizeof(S)) && rows16(p.C, p.Cs, 2, sizeof(S));
+    fms::ssm_step_kernel<S, VEC, U><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), log_L, bc_vec);
+    return check_launch();
+}
 template <typename S>
 int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
     const auto p = ssm_problem<S>(a, 1, 1);
-    int L = 1;
-    while (L < 32 && 4 * L < p.N) L *= 2;
-    const int64_t blocks = (p.channels + 128 / L - 1) / (128 / L);
-    if (blocks > kMaxGrid || p.batch * blocks > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    const unsigned grid = static_cast<unsigned>(p.batch * blocks);
-    if (p.N % 4 == 0 && aligned_to(state, 16) && aligned_to(p.A, 16))
-        fms::ssm_step_kernel<S, true><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), L, static_cast<int>(blocks));
-    else
-        fms::ssm_step_kernel<S, false><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), L, static_cast<int>(blocks));
-    return check_launch();
+    if (p.groups > 65535) return FMS_ERR_TOO_LARGE;
+    int log_L = 0;
+    while (log_L < 5 && (8 << log_L) < p.N) ++log_L;
+    const bool vec = p.N % 8 == 0 && aligned_to(state, 16) && aligned_to(p.A, 16);
+    const bool many = (p.batch * p.channels << log_L) >= env_int("X_MANY", 148 * 1024);
+    if (vec) return many ? launch_ssm_step_u<S, true, 2>(p, state, pool, slots, out, log_L, st)
+                         : launch_ssm_step_u<S, true, 1>(p, state, pool, slots, out, log_L, st);
+    return launch_ssm_step_u<S, false, 1>(p, state, pool, slots, out, log_L, st);
 }
 
 // ------------------------------------------------------------------------------- filter ----

@@ -965,75 +965,98 @@ __device__ __forceinline__ bool slot_taken(const int64_t *slots, int64_t b, int6
     return __syncthreads_or(seen);
 }
 
-// L lanes share a channel, a lane has 4 consecutive states at a time.  Bound by the states' bytes
-// (8 per state) and, for a few rows, by latency: all loads are issued before the first use.
-template <typename S, bool VEC>
+// Eight consecutive values; `vec`: they are whole and start on a 16-byte boundary.
+template <typename S>
+__device__ __forceinline__ void load_eight(const S *__restrict__ p, bool vec, int left, float (&f)[8]) {
+    if (vec) {
+        if constexpr (sizeof(S) == 4) {
+            const float4 v = reinterpret_cast<const float4 *>(p)[0], w = reinterpret_cast<const float4 *>(p)[1];
+            f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
+        } else {
+            Store<S>::unpack(*reinterpret_cast<const uint4 *>(p), f);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < left ? Store<S>::to_float(p[i]) : 0.f;
+    }
+}
+
+// A block has 128 U / L channels of one row and group.  What a channel needs once (time step, gate) is
+// prepared by one thread per channel in shared memory while the states, asked for before, are on their
+// way; then L lanes share a channel, 8 states a lane (B and C in registers), U channels a thread.  Bound
+// by the states' bytes (8 per state) for many rows, by the latency of one pass for a few: U = 1 there.
+// VEC: states and A come in vectors.
+template <typename S, bool VEC, int U>
 __global__ void __launch_bounds__(128)
 ssm_step_kernel(const SsmProblem<S> p, float *__restrict__ state, int64_t pool, const int64_t *__restrict__ slots,
-                S *__restrict__ out, int L, int blocks) {
-    const int64_t b = blockIdx.x / blocks;
-    const int l = threadIdx.x % L;
-    const int64_t d = static_cast<int64_t>(blockIdx.x % blocks) * (blockDim.x / L) + threadIdx.x / L;
-    const bool live = d < p.channels;
-    const int64_t slot = step_slot(slots, b, pool);
-    const bool use = live && slot >= 0;
-    const int64_t g = live ? d / p.per_group : 0;
-    float x = 0.f, dt = 0.f, z = 0.f, D = 0.f;
-    float h[4] = {}, A[4] = {}, B[4] = {}, C[4] = {};
-    float *hp = state + (slot * p.channels + d) * p.N;
-    const float *Ap = p.A + d * p.N;
-    const S *Bp = p.B + b * p.Bs[0] + g * p.Bs[1], *Cp = p.C + b * p.Cs[0] + g * p.Cs[1];
-    auto fetch = [&](int n) {
-        if constexpr (VEC) {
-            const float4 hv = *reinterpret_cast<const float4 *>(hp + n);
-            const float4 av = __ldg(reinterpret_cast<const float4 *>(Ap + n));
-            h[0] = hv.x, h[1] = hv.y, h[2] = hv.z, h[3] = hv.w;
-            A[0] = av.x, A[1] = av.y, A[2] = av.z, A[3] = av.w;
-        }
+                S *__restrict__ out, int log_L, bool bc_vec) {
+    __shared__ float4 once[128 * U];  // dt log2(e), dt x, D x, gate
+    __shared__ float y_[128 * U];
+    const int L = 1 << log_L, per = 128 >> log_L, l = threadIdx.x & (L - 1), c0 = threadIdx.x >> log_L;
+    const int first = blockIdx.x * per * U, nc = min(per * U, p.per_group - first), g = blockIdx.y;
+    const int64_t d0 = static_cast<int64_t>(g) * p.per_group + first;
+    for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
+        const int64_t slot = step_slot(slots, b, pool);
+        const S *Bp = p.B + b * p.Bs[0] + g * p.Bs[1], *Cp = p.C + b * p.Cs[0] + g * p.Cs[1];
+        float *hp = state + (slot * p.channels + d0 + c0) * p.N;
+        const float *Ap = p.A + (d0 + c0) * p.N;
+        float y[U], h[U][8], A[U][8], B[8], C[8];
+        auto fetch = [&](int n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = n + i < p.N;
-            if (!VEC) {
-                h[i] = in ? hp[n + i] : 0.f;
-                A[i] = in ? Ap[n + i] : 0.f;
-            }
-            B[i] = in ? Store<S>::to_float(Bp[n + i]) : 0.f;
-            C[i] = in ? Store<S>::to_float(Cp[n + i]) : 0.f;
-        }
-    };
-    if (use) {
-        x = Store<S>::to_float(p.x[b * p.xs[0] + d]);
-        dt = Store<S>::to_float(p.delta[b * p.ds[0] + d]) + (p.bias ? p.bias[d] : 0.f);
-        if (p.z) z = Store<S>::to_float(p.z[b * p.zs[0] + d]);
-        if (p.D) D = p.D[d];
-        if (4 * l < p.N) fetch(4 * l);
-    }
-    const bool taken = slot_taken(slots, b, slot);
-    float y = 0.f;
-    if (use && !taken) {
-        if (p.softplus) dt = softplus_f(dt);
-        const float u = dt * x;
-        for (int n = 4 * l; n < p.N; n += 4 * L) {
-            if (n != 4 * l) fetch(n);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h[i] = fmaf(ex2(dt * (A[i] * kLog2e)), h[i], u * B[i]);
-                y = fmaf(C[i], h[i], y);
-            }
-            if constexpr (VEC) {
-                *reinterpret_cast<float4 *>(hp + n) = make_float4(h[0], h[1], h[2], h[3]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n + i < p.N) hp[n + i] = h[i];
+            for (int k = 0; k < U; ++k)
+                if (c0 + k * per < nc) {
+                    load_eight(hp + k * per * p.N + n, VEC, p.N - n, h[k]);
+                    load_eight(Ap + k * per * p.N + n, VEC, p.N - n, A[k]);
+                }
+            load_eight(Bp + n, bc_vec, p.N - n, B);
+            load_eight(Cp + n, bc_vec, p.N - n, C);
+        };
+        if (slot >= 0) {
+            if (8 * l < p.N) fetch(8 * l);
+            for (int c = threadIdx.x; c < nc; c += 128) {
+                const int64_t d = d0 + c;
+                const float x = Store<S>::to_float(p.x[b * p.xs[0] + d]), z = p.z ? Store<S>::to_float(p.z[b * p.zs[0] + d]) : 0.f;
+                float dt = Store<S>::to_float(p.delta[b * p.ds[0] + d]) + (p.bias ? p.bias[d] : 0.f);
+                if (p.softplus) dt = softplus_f(dt);
+                once[c] = make_float4(dt * kLog2e, dt * x, p.D ? p.D[d] * x : 0.f, p.z ? z * sigmoid_f(z) : 1.f);
             }
         }
-    }
-    for (int k = 1; k < L; k *= 2) y += __shfl_xor_sync(kFullMask, y, k);
-    if (live && l == 0) {
-        y = fmaf(D, x, y);
-        if (p.z) y *= z * sigmoid_f(z);
-        out[b * p.channels + d] = from_float<S>(use && !taken ? y : 0.f);
+        const bool use = !slot_taken(slots, b, slot) && slot >= 0;  // the block's barrier too
+        if (use) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) y[k] = 0.f;
+            for (int n = 8 * l; n < p.N; n += 8 * L) {
+                if (n != 8 * l) fetch(n);
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (c0 + k * per < nc) {
+                        const float2 v = *reinterpret_cast<const float2 *>(&once[c0 + k * per]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            h[k][i] = fmaf(ex2(v.x * A[k][i]), h[k][i], v.y * B[i]);
+                            y[k] = fmaf(C[i], h[k][i], y[k]);
+                        }
+                        float *to = hp + k * per * p.N + n;
+                        if constexpr (VEC) {
+                            reinterpret_cast<float4 *>(to)[0] = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
+                            reinterpret_cast<float4 *>(to)[1] = make_float4(h[k][4], h[k][5], h[k][6], h[k][7]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (n + i < p.N) to[i] = h[k][i];
+                        }
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                for (int i = 1; i < L; i *= 2) y[k] += __shfl_xor_sync(kFullMask, y[k], i);
+                if (l == 0) y_[c0 + k * per] = y[k];
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < nc; c += 128)
+            out[b * p.channels + d0 + c] = from_float<S>(use ? (y_[c] + once[c].z) * once[c].w : 0.f);
+        __syncthreads();
     }
 }
 

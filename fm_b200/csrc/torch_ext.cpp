@@ -15,6 +15,7 @@
 // gates (B,M,L) x tokens (B,D,L) -> states (B,M,D,L) with the 1 - gate token weight.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "fm_scan_b200.h"
@@ -629,6 +630,162 @@ static at::Tensor short_conv_step(const at::Tensor &x, const at::Tensor &state, 
     return out;
 }
 
+// ---- what Python calls: casts, copies of strided tensors and autograd are done here, where they cost less
+// than in Python.
+
+// a tensor with a contiguous last axis; parameters in fp32; indexes in int64
+static at::Tensor rows_of(const at::Tensor &t) {
+    return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+static OptTensor rows_of(const OptTensor &t) { return given(t) ? OptTensor(rows_of(*t)) : OptTensor(); }
+static at::Tensor fp32_of(const at::Tensor &t) {
+    if (t.scalar_type() == at::kFloat && t.is_contiguous()) return t;
+    TORCH_CHECK(t.is_floating_point(), "parameters and states must be floating point");
+    return t.to(at::kFloat).contiguous();
+}
+static OptTensor fp32_of(const OptTensor &t) { return given(t) ? OptTensor(fp32_of(*t)) : OptTensor(); }
+static OptTensor index_of(const OptTensor &t) {
+    return given(t) && t->scalar_type() == at::kInt ? OptTensor(t->to(at::kLong)) : t;
+}
+static bool needs(const at::Tensor &t) { return t.requires_grad(); }
+static bool needs(const OptTensor &t) { return given(t) && t->requires_grad(); }
+template <typename... Ts>
+static bool wants_grad(const Ts &...ts) {
+    return at::GradMode::is_enabled() && (needs(ts) || ...);
+}
+static at::Tensor value(const OptTensor &t) { return given(t) ? *t : at::Tensor(); }
+static OptTensor maybe(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that cannot be differentiated again: when a graph of the backward is asked for, going
+// through it raises.
+static variable_list first_order(variable_list grads, const char *what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list some;
+    for (const at::Tensor &g : grads)
+        if (g.defined()) some.push_back(g);
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative",
+                                                                 static_cast<int64_t>(some.size()));
+    for (at::Tensor &g : some) g.requires_grad_(true);
+    some = (*error)(std::move(some));
+    size_t k = 0;
+    for (at::Tensor &g : grads)
+        if (g.defined()) g = some[k++];
+    return grads;
+}
+
+// Saved for backward: the inputs and the states in front of every 64th position; the others are recomputed.
+struct SsmScan : torch::autograd::Function<SsmScan> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &delta, const at::Tensor &A,
+                                 const at::Tensor &B, const at::Tensor &C, const OptTensor &D, const OptTensor &z,
+                                 const OptTensor &bias, const OptTensor &h0, const OptTensor &lengths, bool softplus,
+                                 bool want_last) {
+        auto [out, last, ck] = ssm_forward(x, delta, A, B, C, D, z, bias, h0, lengths, softplus, want_last, true);
+        ctx->save_for_backward({x, delta, A, B, C, value(D), value(z), value(bias), value(h0), value(lengths), *ck});
+        ctx->saved_data["softplus"] = softplus;
+        ctx->set_materialize_grads(false);
+        if (want_last) return {out, *last};
+        return {out};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list r;
+        {
+            const at::AutoGradMode off(false);
+            const at::Tensor up = g[0].defined() ? g[0].contiguous() : at::zeros(s[0].sizes(), s[0].options());
+            const OptTensor last = g.size() > 1 && g[1].defined() ? OptTensor(g[1].contiguous()) : OptTensor();
+            for (const OptTensor &t : ssm_backward(s[0], s[1], s[2], s[3], s[4], maybe(s[5]), maybe(s[6]), maybe(s[7]), maybe(s[8]),
+                                                   maybe(s[9]), ctx->saved_data["softplus"].toBool(), s[10], up, last))
+                r.push_back(value(t));
+        }
+        r = first_order(std::move(r), "ssm_scan");
+        r.resize(12);
+        return r;
+    }
+};
+
+static py::object ssm_scan(const at::Tensor &tokens, const at::Tensor &delta, const at::Tensor &A, const at::Tensor &B,
+                           const at::Tensor &C, const OptTensor &D, const OptTensor &z, const OptTensor &bias,
+                           const OptTensor &initial_state, bool softplus, const OptTensor &lengths, bool want_last) {
+    const at::Tensor x_ = rows_of(tokens), d_ = rows_of(delta), A_ = fp32_of(A), B_ = rows_of(B), C_ = rows_of(C);
+    const OptTensor D_ = fp32_of(D), z_ = rows_of(z), b_ = fp32_of(bias), h_ = fp32_of(initial_state), n_ = index_of(lengths);
+    at::Tensor out;
+    OptTensor last;
+    if (wants_grad(x_, d_, A_, B_, C_, D_, z_, b_, h_)) {
+        const variable_list r = SsmScan::apply(x_, d_, A_, B_, C_, D_, z_, b_, h_, n_, softplus, want_last);
+        out = r[0];
+        if (want_last) last = r[1];
+    } else {
+        std::tie(out, last, std::ignore) = ssm_forward(x_, d_, A_, B_, C_, D_, z_, b_, h_, n_, softplus, want_last, false);
+    }
+    if (want_last) return py::make_tuple(out, *last);
+    return py::cast(out);
+}
+
+// Saved for backward: the inputs; what stands before the activation is recomputed.
+struct ShortConv : torch::autograd::Function<ShortConv> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias,
+                                 const OptTensor &x0, const OptTensor &lengths, bool silu, bool want_last) {
+        auto [out, last] = short_conv_forward(x, weight, bias, x0, lengths, silu, want_last);
+        ctx->save_for_backward({x, weight, value(bias), value(x0), value(lengths)});
+        ctx->saved_data["silu"] = silu;
+        ctx->set_materialize_grads(false);
+        if (want_last) return {out, *last};
+        return {out};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list r;
+        {
+            const at::AutoGradMode off(false);
+            const at::Tensor up = g[0].defined() ? g[0].contiguous() : at::zeros(s[0].sizes(), s[0].options());
+            const OptTensor last = g.size() > 1 && g[1].defined() ? OptTensor(g[1].contiguous()) : OptTensor();
+            for (const OptTensor &t : short_conv_backward(s[0], s[1], maybe(s[2]), maybe(s[3]), maybe(s[4]),
+                                                          ctx->saved_data["silu"].toBool(), up, last))
+                r.push_back(value(t));
+        }
+        r = first_order(std::move(r), "short_conv");
+        r.resize(7);
+        return r;
+    }
+};
+
+static py::object short_conv(const at::Tensor &tokens, const at::Tensor &weight, const OptTensor &bias,
+                             const OptTensor &initial_state, bool silu, const OptTensor &lengths, bool want_last) {
+    const at::Tensor x_ = rows_of(tokens), w_ = fp32_of(weight);
+    const OptTensor b_ = fp32_of(bias), n_ = index_of(lengths);
+    const OptTensor i_ = given(initial_state) ? OptTensor(initial_state->contiguous()) : OptTensor();
+    at::Tensor out;
+    OptTensor last;
+    if (wants_grad(x_, w_, b_, i_)) {
+        const variable_list r = ShortConv::apply(x_, w_, b_, i_, n_, silu, want_last);
+        out = r[0];
+        if (want_last) last = r[1];
+    } else {
+        std::tie(out, last) = short_conv_forward(x_, w_, b_, i_, n_, silu, want_last);
+    }
+    if (want_last) return py::make_tuple(out, *last);
+    return py::cast(out);
+}
+
+static at::Tensor ssm_step_op(const at::Tensor &x, const at::Tensor &delta, const at::Tensor &state, const at::Tensor &A,
+                              const at::Tensor &B, const at::Tensor &C, const OptTensor &D, const OptTensor &z,
+                              const OptTensor &bias, bool softplus, const OptTensor &slots) {
+    TORCH_CHECK(!wants_grad(x, delta, state, A, B, C, D, z, bias),
+                "ssm_step has no gradient: call it under torch.no_grad() or on detached tensors");
+    return ssm_step(rows_of(x), rows_of(delta), state, fp32_of(A), rows_of(B), rows_of(C), fp32_of(D), rows_of(z), fp32_of(bias),
+                    softplus, index_of(slots));
+}
+
+static at::Tensor short_conv_step_op(const at::Tensor &x, const at::Tensor &state, const at::Tensor &weight, const OptTensor &bias,
+                                     bool silu, const OptTensor &slots) {
+    TORCH_CHECK(!wants_grad(x, state, weight, bias),
+                "short_conv_step has no gradient: call it under torch.no_grad() or on detached tensors");
+    return short_conv_step(rows_of(x), state, fp32_of(weight), fp32_of(bias), silu, index_of(slots));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "fm_scan for B200: torch shim over the C ABI libfm_scan_b200.so";
     m.def("fm_scan_forward", &fm_scan_forward, "scan forward (writes and returns out)");
@@ -640,11 +797,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fm_memory_forward_train", &fm_memory_forward_train, "layer forward: output + normalised states");
     m.def("fm_memory_backward", &fm_memory_backward, "layer backward with the state gradient generated in-kernel");
     m.def("fm_memory_readout", &fm_memory_readout, "layer read-out without materialising the states");
+    m.def("ssm_scan", &ssm_scan, "state-space scan, differentiable: out or (out, last state)");
+    m.def("ssm_step", &ssm_step_op, "state-space scan of one token, states advanced in place");
+    m.def("short_conv", &short_conv, "causal filter, differentiable: out or (out, last inputs)");
+    m.def("short_conv_step", &short_conv_step_op, "causal filter of one token, state shifted in place");
     m.def("ssm_forward", &ssm_forward, "state-space scan forward: out, last state, checkpoints");
     m.def("ssm_backward", &ssm_backward, "state-space scan backward: gradients of every input");
-    m.def("ssm_step", &ssm_step, "state-space scan of one token, states advanced in place");
     m.def("short_conv_forward", &short_conv_forward, "causal filter forward: out, last inputs");
     m.def("short_conv_backward", &short_conv_backward, "causal filter backward: gradients of every input");
-    m.def("short_conv_step", &short_conv_step, "causal filter of one token, state shifted in place");
     m.def("abi_version", []() { return fms_version(); });
 }
