@@ -1,48 +1,14 @@
-// C ABI of the selective state-space scan and its causal filter (see include/fm_scan_b200.h): argument
+// C ABI of the selective state-space scan (see include/fm_scan_b200.h): argument
 // checks, launch shapes, launches.  No allocation, no synchronisation, no torch.
 #include "fm_scan_b200.h"
 
 #include <algorithm>
 #include <cstdlib>
 
-#include "conv_kernels.cuh"
+#include "capi_common.cuh"
 #include "ssm_kernels.cuh"
 
-#define FMS_EXPORT extern "C" __attribute__((visibility("default")))
-
-namespace fms {
-int record_cuda_error(cudaError_t e);  // fm_scan_capi.cu: this thread's fms_last_cuda_error
-}
-
 namespace {
-
-constexpr int64_t kMaxGrid = 0x7fffffff;
-constexpr size_t kMaxSmem = 227 * 1024;  // of a CTA on sm_100
-
-inline int check_launch() { return fms::record_cuda_error(cudaGetLastError()); }
-inline bool dtype_ok(int d) { return d == FMS_F32 || d == FMS_F16 || d == FMS_BF16; }
-inline int64_t elem_size(int d) { return d == FMS_F32 ? 4 : 2; }
-inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-
-// a * b * c * ... with every product below 2^59, so that byte offsets fit int64
-bool product_ok(std::initializer_list<int64_t> v) {
-    int64_t p = 1;
-    for (int64_t k : v) {
-        if (k < 0) return false;
-        if (k && p > (int64_t{1} << 59) / k) return false;
-        p *= k ? k : 1;
-    }
-    return true;
-}
-
-// every row of a tensor with these element strides starts on a 16-byte boundary
-bool rows16(const void *p, const int64_t *stride, int n, int64_t es) {
-    if (!aligned_to(p, 16)) return false;
-    for (int i = 0; i < n; ++i)
-        if (stride[i] * es % 16) return false;
-    return true;
-}
 
 int ssm_check(const fms_ssm_args *a) {
     if (!a) return FMS_ERR_NULL_POINTER;
@@ -143,21 +109,19 @@ int allow_smem(Kernel kernel, size_t bytes) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
-__global__ void fill_kernel(const float *__restrict__ src, float *__restrict__ dst, int64_t n) {
+// out[i] = sum over `count` slices of `stride` floats, in order
+__global__ void sum_slices_kernel(const float *__restrict__ part, float *__restrict__ out, int64_t n, int64_t count,
+                                  int64_t stride) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i < n) dst[i] = src ? src[i] : 0.f;
+    if (i >= n) return;
+    float v = 0.f;
+    for (int64_t k = 0; k < count; ++k) v += part[k * stride + i];
+    out[i] = v;
 }
-int copy_or_zero(const float *src, float *dst, int64_t n, cudaStream_t st) {
-    if (!dst || n == 0) return FMS_OK;
-    if ((n + 255) / 256 > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    fill_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(src, dst, n);
-    return check_launch();
-}
-
 int sum_slices(const float *part, float *out, int64_t n, int64_t count, int64_t stride, cudaStream_t st) {
     if (!out || n == 0) return FMS_OK;
     if ((n + 127) / 128 > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    fms::sum_slices_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, st>>>(part, out, n, count, stride);
+    sum_slices_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, st>>>(part, out, n, count, stride);
     return check_launch();
 }
 
@@ -235,123 +199,9 @@ int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int
     return launch_ssm_step_u<S, false, 1>(p, state, pool, slots, out, log_L, st);
 }
 
-// ------------------------------------------------------------------------------- filter ----
-
-int conv_check(const fms_conv_args *a) {
-    if (!a) return FMS_ERR_NULL_POINTER;
-    if (!dtype_ok(a->dtype)) return FMS_ERR_BAD_DTYPE;
-    if (a->batch < 0 || a->channels < 0 || a->T < 0 || a->taps < 2 || a->taps > 8) return FMS_ERR_BAD_SHAPE;
-    if (a->T > 0x7fffffff - 4096) return FMS_ERR_TOO_LARGE;
-    if (!product_ok({a->batch, a->channels, std::max<int64_t>(a->T, 16)})) return FMS_ERR_BAD_SHAPE;
-    return FMS_OK;
-}
-int conv_pointers(const fms_conv_args *a) {
-    if (!a->weight || (a->T && !a->tokens)) return FMS_ERR_NULL_POINTER;
-    const size_t es = elem_size(a->dtype);
-    if (!aligned_to(a->tokens, es) || !aligned_to(a->x0, es) || !aligned_to(a->weight, 4) || !aligned_to(a->bias, 4) ||
-        !aligned_to(a->lengths, 8))
-        return FMS_ERR_MISALIGNED;
-    return FMS_OK;
-}
-bool conv_aligned(const fms_conv_args *a) {
-    const int64_t es = elem_size(a->dtype);
-    return a->T * es % 16 == 0 && rows16(a->tokens, a->tokens_stride, 2, es);
-}
-
-int conv_lanes(int64_t T) {
-    int lpr = 1;
-    while (lpr < 32 && lpr * 8 < T) lpr *= 2;
-    return lpr;
-}
-int64_t conv_chunks(int64_t T) {
-    const int64_t span = static_cast<int64_t>(conv_lanes(T)) * 8 * fms::kConvUnroll;
-    return std::max<int64_t>(1, (T + span - 1) / span);
-}
-
-template <typename S>
-fms::ConvProblem<S> conv_problem(const fms_conv_args *a) {
-    fms::ConvProblem<S> p;
-    p.x = static_cast<const S *>(a->tokens);
-    std::copy_n(a->tokens_stride, 2, p.xs);
-    p.weight = a->weight, p.bias = a->bias, p.x0 = static_cast<const S *>(a->x0), p.lengths = a->lengths;
-    p.batch = a->batch, p.channels = a->channels, p.chunks = conv_chunks(a->T);
-    p.T = static_cast<int>(a->T), p.lpr = conv_lanes(a->T), p.silu = a->silu != 0;
-    return p;
-}
-template <typename S>
-int64_t conv_grid(const fms::ConvProblem<S> &p) {
-    const int64_t per = 32 / p.lpr, units = (p.batch * p.channels + per - 1) / per * p.chunks;
-    return (units + fms::kConvWarps - 1) / fms::kConvWarps;
-}
-
-template <typename S, int K, bool ALIGNED>
-int launch_conv_forward(const fms_conv_args *a, void *out, void *x_last, cudaStream_t st) {
-    const auto p = conv_problem<S>(a);
-    if (conv_grid(p) > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    fms::conv_forward_kernel<S, K, ALIGNED><<<static_cast<unsigned>(conv_grid(p)), fms::kConvWarps * 32, 0, st>>>(
-        p, static_cast<S *>(out), static_cast<S *>(x_last));
-    return check_launch();
-}
-
-template <typename S, int K, bool ALIGNED>
-int launch_conv_backward(const fms_conv_args *a, const void *dout, const void *dlast, void *dx, float *dw, float *db,
-                         void *dx0, float *part, cudaStream_t st) {
-    const auto p = conv_problem<S>(a);
-    if (conv_grid(p) > kMaxGrid || (p.channels + 3) / 4 > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    fms::conv_backward_kernel<S, K, ALIGNED><<<static_cast<unsigned>(conv_grid(p)), fms::kConvWarps * 32, 0, st>>>(
-        p, static_cast<const S *>(dout), static_cast<const S *>(dlast), static_cast<S *>(dx), static_cast<S *>(dx0), part);
-    if (int rc = check_launch()) return rc;
-    fms::conv_weight_kernel<K><<<static_cast<unsigned>((p.channels + 3) / 4), 128, 0, st>>>(part, dw, db, p.batch,
-                                                                                         p.channels, p.chunks);
-    return check_launch();
-}
-
-template <typename S, int K>
-int launch_conv_step(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
-    const auto p = conv_problem<S>(a);
-    const int64_t blocks = (p.channels + 127) / 128;
-    if (blocks > kMaxGrid || p.batch * blocks > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    fms::conv_step_kernel<S, K><<<static_cast<unsigned>(p.batch * blocks), 128, 0, st>>>(
-        p, static_cast<S *>(state), pool, slots, static_cast<S *>(out), static_cast<int>(blocks));
-    return check_launch();
-}
-
 }  // namespace
 
-#define FMS_BY_TYPE(dtype, CALL)                                         \
-    switch (dtype) {                                                     \
-        case FMS_F32: { using S = float; return CALL; }                  \
-        case FMS_F16: { using S = __half; return CALL; }                 \
-        default: { using S = __nv_bfloat16; return CALL; }               \
-    }
-#define FMS_BY_TAPS(taps, CALL)                                          \
-    switch (taps) {                                                      \
-        case 2: { constexpr int K = 2; return CALL; }                    \
-        case 3: { constexpr int K = 3; return CALL; }                    \
-        case 4: { constexpr int K = 4; return CALL; }                    \
-        case 5: { constexpr int K = 5; return CALL; }                    \
-        case 6: { constexpr int K = 6; return CALL; }                    \
-        case 7: { constexpr int K = 7; return CALL; }                    \
-        default: { constexpr int K = 8; return CALL; }                   \
-    }
-
 namespace {
-template <typename S>
-int conv_forward_t(const fms_conv_args *a, void *out, void *x_last, cudaStream_t st) {
-    if (conv_aligned(a) && aligned_to(out, 16)) FMS_BY_TAPS(a->taps, (launch_conv_forward<S, K, true>(a, out, x_last, st)));
-    FMS_BY_TAPS(a->taps, (launch_conv_forward<S, K, false>(a, out, x_last, st)));
-}
-template <typename S>
-int conv_backward_t(const fms_conv_args *a, const void *dout, const void *dlast, void *dx, float *dw, float *db, void *dx0,
-                    float *part, cudaStream_t st) {
-    if (conv_aligned(a) && aligned_to(dout, 16) && aligned_to(dx, 16))
-        FMS_BY_TAPS(a->taps, (launch_conv_backward<S, K, true>(a, dout, dlast, dx, dw, db, dx0, part, st)));
-    FMS_BY_TAPS(a->taps, (launch_conv_backward<S, K, false>(a, dout, dlast, dx, dw, db, dx0, part, st)));
-}
-template <typename S>
-int conv_step_t(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
-    FMS_BY_TAPS(a->taps, (launch_conv_step<S, K>(a, state, pool, slots, out, st)));
-}
 template <typename S>
 int ssm_forward_t(const fms_ssm_args *a, void *out, float *h_last, float *ck, cudaStream_t st) {
     return ssm_aligned(a) && aligned_to(out, 16) ? launch_ssm_forward<S, true>(a, out, h_last, ck, st)
@@ -437,56 +287,4 @@ FMS_EXPORT int fms_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, c
     if (!aligned_to(state, 4) || !aligned_to(slots, 8) || !aligned_to(out, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     FMS_BY_TYPE(a->dtype, (launch_ssm_step<S>(a, state, pool, slots, out, st)));
-}
-
-FMS_EXPORT int fms_conv_forward(const fms_conv_args *a, void *out, void *x_last, fms_stream_t stream) {
-    if (int rc = conv_check(a)) return rc;
-    if (a->batch == 0 || a->channels == 0) return FMS_OK;
-    if (int rc = conv_pointers(a)) return rc;
-    if (a->T && !out) return FMS_ERR_NULL_POINTER;
-    if (!aligned_to(out, elem_size(a->dtype)) || !aligned_to(x_last, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
-    if (a->T == 0 && !x_last) return FMS_OK;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    FMS_BY_TYPE(a->dtype, (conv_forward_t<S>(a, out, x_last, st)));
-}
-
-FMS_EXPORT size_t fms_conv_backward_workspace_bytes(const fms_conv_args *a) {
-    if (conv_check(a) != FMS_OK || a->batch == 0 || a->channels == 0) return 0;
-    return round256(sizeof(float) * a->batch * a->channels * conv_chunks(a->T) * (a->taps + 1));
-}
-
-FMS_EXPORT int fms_conv_backward(const fms_conv_args *a, const void *grad_out, const void *grad_last, void *grad_tokens,
-                                 float *grad_weight, float *grad_bias, void *grad_x0, void *workspace,
-                                 size_t workspace_bytes, fms_stream_t stream) {
-    if (int rc = conv_check(a)) return rc;
-    if (a->channels == 0) return FMS_OK;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!grad_weight) return FMS_ERR_NULL_POINTER;
-    if (!aligned_to(grad_weight, 4) || !aligned_to(grad_bias, 4)) return FMS_ERR_MISALIGNED;
-    if (a->batch == 0) {
-        if (int rc = copy_or_zero(nullptr, grad_weight, a->channels * a->taps, st)) return rc;
-        return copy_or_zero(nullptr, grad_bias, a->channels, st);
-    }
-    if (int rc = conv_pointers(a)) return rc;
-    if (a->T && (!grad_out || !grad_tokens)) return FMS_ERR_NULL_POINTER;
-    for (const void *p : {grad_out, grad_last, static_cast<const void *>(grad_tokens), static_cast<const void *>(grad_x0)})
-        if (!aligned_to(p, elem_size(a->dtype))) return FMS_ERR_MISALIGNED;
-    if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < fms_conv_backward_workspace_bytes(a))
-        return FMS_ERR_WORKSPACE;
-    FMS_BY_TYPE(a->dtype, (conv_backward_t<S>(a, grad_out, grad_last, grad_tokens, grad_weight, grad_bias, grad_x0,
-                                              static_cast<float *>(workspace), st)));
-}
-
-FMS_EXPORT int fms_conv_step(const fms_conv_args *a, void *state, int64_t pool, const int64_t *slots, void *out,
-                             fms_stream_t stream) {
-    if (int rc = conv_check(a)) return rc;
-    if (a->T != 1 || pool < 0 || (!slots && pool < a->batch)) return FMS_ERR_BAD_SHAPE;
-    if (!product_ok({pool, a->channels, 8})) return FMS_ERR_BAD_SHAPE;
-    if (a->batch == 0 || a->channels == 0) return FMS_OK;
-    if (int rc = conv_pointers(a)) return rc;
-    if (!out || (pool && !state)) return FMS_ERR_NULL_POINTER;
-    if (!aligned_to(state, elem_size(a->dtype)) || !aligned_to(slots, 8) || !aligned_to(out, elem_size(a->dtype)))
-        return FMS_ERR_MISALIGNED;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    FMS_BY_TYPE(a->dtype, (conv_step_t<S>(a, state, pool, slots, out, st)));
 }

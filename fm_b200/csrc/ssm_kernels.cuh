@@ -940,16 +940,6 @@ __global__ void ssm_bc_kernel(const float *__restrict__ part, S *__restrict__ dB
     }
 }
 
-// out[i] = sum over `count` slices of `stride` floats, in order
-__global__ void sum_slices_kernel(const float *__restrict__ part, float *__restrict__ out, int64_t n, int64_t count,
-                                  int64_t stride) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    float v = 0.f;
-    for (int64_t k = 0; k < count; ++k) v += part[k * stride + i];
-    out[i] = v;
-}
-
 // ---------------------------------------------------------------- one token ------------------
 // Row b's place in the pool, or -1 for padding.  A slot that an earlier row names belongs to that row:
 // every thread looks at its share of the earlier rows and the block votes, while the loads of the
