@@ -53,7 +53,7 @@ class ConvArgs(ctypes.Structure):
 
 _SSM, _CONV, _SIZE = ctypes.POINTER(SsmArgs), ctypes.POINTER(ConvArgs), ctypes.c_size_t
 SIGNATURES.update({
-    "fms_ssm_forward": [_SSM, _P, _P, _P, _P],
+    "fms_ssm_forward": [_SSM, _P, _P, _P, _P, _SIZE, _P],
     "fms_ssm_backward": [_SSM, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SIZE, _P],
     "fms_ssm_step": [_SSM, _P, _I64, _P, _P, _P],
     "fms_conv_forward": [_CONV, _P, _P, _P],
@@ -96,7 +96,7 @@ def lib() -> ctypes.CDLL:
         L.fms_plain_split_workspace_bytes.argtypes = [_I64, _I64, _I]
         L.fms_fm_backward_workspace_bytes.restype = ctypes.c_size_t
         L.fms_fm_backward_workspace_bytes.argtypes = [_I64, _I64, _I64, _I64, _I]
-        for name, args in (("fms_ssm_checkpoint_bytes", _SSM), ("fms_ssm_backward_workspace_bytes", _SSM),
+        for name, args in (("fms_ssm_checkpoint_bytes", _SSM), ("fms_ssm_forward_workspace_bytes", _SSM), ("fms_ssm_backward_workspace_bytes", _SSM),
                            ("fms_conv_backward_workspace_bytes", _CONV)):
             fn = getattr(L, name)
             fn.restype, fn.argtypes = _SIZE, [args]

@@ -43,8 +43,79 @@ bool ssm_aligned(const fms_ssm_args *a) {
            rows16(a->C, a->C_stride, 3, es);
 }
 
+inline int padded_states(const fms_ssm_args *a) {
+    return static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
+}
+
+int env_int(const char *name, int dflt) { const char *s = std::getenv(name); return s ? std::atoi(s) : dflt; }
+// shared memory of a CTA: as the kernels lay it out
+template <typename F>
+size_t by_width(const fms_ssm_args *a, F f) { return a->dtype == FMS_F32 ? f(float{}) : f(__half{}); }
+size_t ssm_fwd_smem(const fms_ssm_args *a, int cw) {
+    return by_width(a, [&](auto t) {
+        using S = decltype(t);
+        return fms::ssm_bc_bytes<S>() + fms::kSsmFwdWarps * fms::ssm_fwd_warp_bytes<S>(cw, padded_states(a));
+    });
+}
+size_t ssm_bwd_smem(const fms_ssm_args *a, int cw) {
+    return sizeof(float) * fms::kSsmBwdWarps * 64 * 32 + by_width(a, [&](auto t) {
+               using S = decltype(t);
+               return fms::ssm_bc_bytes<S>() + fms::kSsmBwdWarps * fms::ssm_bwd_warp_bytes<S>(cw, padded_states(a));
+           });
+}
+size_t ssm_carry_smem(const fms_ssm_args *a, int cw) {
+    return by_width(a, [&](auto t) {
+        using S = decltype(t);
+        return fms::ssm_bc_bytes<S>() + fms::kSsmFwdWarps * fms::ssm_carry_warp_bytes<S>(cw, padded_states(a));
+    });
+}
+
+// How the work is cut: channels of a warp, pieces of time.  More channels spread a tile's B, C and barriers
+// over more work (and, backward, shrink the partial sums of their gradients); fewer, and more pieces of
+// time, give more CTAs, but pieces cost a first pass over the data, a fold and two launches.  The cut with
+// the least expected time is taken.  Measured on B200 (16-bit types, N = 16): a CTA's tile takes
+// (channels of a warp + 1.5) x `unit[n - 1]` microseconds with n CTAs on an SM; a cut time takes `again`
+// as long, plus `fixed` for its launches.
+struct CutCosts {
+    int warps, per_sm;
+    double unit[3], again, fixed;
+};
+constexpr CutCosts kFwdCosts{fms::kSsmFwdWarps, 3, {0.68, 0.80, 1.08}, 1.7, 12};
+constexpr CutCosts kBwdCosts{fms::kSsmBwdWarps, 1, {2.14, 2.14, 2.14}, 1.32, 14};
+
+struct SsmCut {
+    int cw, segs, seg_tiles;
+};
+SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const fms_ssm_args *, int), int force_cw, int force_segs) {
+    const int64_t per = a->channels / a->groups, sms = 148;
+    const int tiles = static_cast<int>((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
+    SsmCut best{1, 1, tiles};
+    double least = 0;
+    for (int cw = 1; cw <= 8; ++cw) {
+        const size_t bytes = smem(a, cw);
+        if (bytes > kMaxSmem) break;
+        if (force_cw && cw != force_cw) continue;
+        const int64_t ctas = a->batch * a->groups * ((per + cw * k.warps - 1) / (cw * k.warps));
+        const int64_t most = std::min<int64_t>(k.per_sm, static_cast<int64_t>((kMaxSmem + 1024) / (bytes + 1024)));
+        for (int waves = 0; waves <= 4; ++waves) {  // 0: time is not cut; else as many pieces as fill the waves
+            int64_t segs = waves ? std::min<int64_t>(tiles, waves * most * sms / ctas) : 1;
+            if (force_segs) segs = std::min(tiles, force_segs);
+            if (segs < 1 || (waves && segs < 2 && !force_segs)) continue;
+            const int64_t len = (tiles + segs - 1) / segs;
+            segs = (tiles + len - 1) / len;
+            const int64_t full = ctas * segs / (most * sms), rest = (ctas * segs - full * most * sms + sms - 1) / sms;
+            double t = (full * k.unit[most - 1] + (rest ? k.unit[rest - 1] : 0)) * len * (cw + 1.5);
+            if (segs > 1) t = t * k.again + k.fixed;
+            if (least == 0 || t < least) best = SsmCut{cw, static_cast<int>(segs), static_cast<int>(len)}, least = t;
+        }
+    }
+    return best;
+}
+SsmCut ssm_fwd_cut(const fms_ssm_args *a) { return best_cut(a, kFwdCosts, ssm_fwd_smem, env_int("X_FCW", 0), env_int("X_FSEG", 0)); }
+SsmCut ssm_bwd_cut(const fms_ssm_args *a) { return best_cut(a, kBwdCosts, ssm_bwd_smem, env_int("X_BCW", 0), env_int("X_BSEG", 0)); }
+
 template <typename S>
-fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, int cw, int warps) {
+fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, const SsmCut &cut, int warps) {
     fms::SsmProblem<S> p;
     p.x = static_cast<const S *>(a->tokens), p.delta = static_cast<const S *>(a->delta), p.z = static_cast<const S *>(a->z);
     p.B = static_cast<const S *>(a->B), p.C = static_cast<const S *>(a->C);
@@ -58,50 +129,14 @@ fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, int cw, int warps) {
     p.T = static_cast<int>(a->T), p.N = static_cast<int>(a->states);
     p.NP = (p.N + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB;
     p.per_group = static_cast<int>(a->channels / a->groups);
-    p.cw = cw;
-    p.chunks = (p.per_group + cw * warps - 1) / (cw * warps);
+    p.cw = cut.cw;
+    p.segs = cut.segs;
+    p.seg_tiles = cut.seg_tiles;
+    p.chunks = (p.per_group + p.cw * warps - 1) / (p.cw * warps);
     p.tiles = static_cast<int>((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
     p.softplus = a->delta_softplus != 0;
     return p;
 }
-
-inline int padded_states(const fms_ssm_args *a) {
-    return static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
-}
-
-// shared memory of a CTA: as the kernels lay it out
-size_t ssm_fwd_smem(const fms_ssm_args *a, int cw) {
-    return a->dtype == FMS_F32
-               ? fms::ssm_bc_bytes<float>() + fms::kSsmFwdWarps * fms::ssm_fwd_warp_bytes<float>(cw, padded_states(a))
-               : fms::ssm_bc_bytes<__half>() + fms::kSsmFwdWarps * fms::ssm_fwd_warp_bytes<__half>(cw, padded_states(a));
-}
-size_t ssm_bwd_smem(const fms_ssm_args *a, int cw) {
-    const size_t red = sizeof(float) * fms::kSsmBwdWarps * 64 * 32;
-    return red + (a->dtype == FMS_F32
-                      ? fms::ssm_bc_bytes<float>() + fms::kSsmBwdWarps * fms::ssm_bwd_warp_bytes<float>(cw, padded_states(a))
-                      : fms::ssm_bc_bytes<__half>() + fms::kSsmBwdWarps * fms::ssm_bwd_warp_bytes<__half>(cw, padded_states(a)));
-}
-
-// Channels of a warp.  More of them spread a tile's B, C and barriers over more work (and, backward,
-// shrink the partial sums of their gradients); fewer give more warps.  The time is taken as the number
-// of waves times the channels of a warp plus the share of a channel that a tile costs on its own.
-int best_cw(const fms_ssm_args *a, int warps, int most, int per_sm, double own, size_t (*smem)(const fms_ssm_args *, int)) {
-    const int64_t per = a->channels / a->groups;
-    int best = 1;
-    double least = 0;
-    for (int cw = 1; cw <= most; ++cw) {
-        const size_t bytes = smem(a, cw);
-        if (bytes > kMaxSmem) break;
-        const int64_t ctas = a->batch * a->groups * ((per + cw * warps - 1) / (cw * warps));
-        const int64_t room = 148 * std::min<int64_t>(per_sm, static_cast<int64_t>((kMaxSmem + 1024) / (bytes + 1024)));
-        const double t = static_cast<double>((ctas + room - 1) / room) * (cw + own);
-        if (cw == 1 || t < least) best = cw, least = t;
-    }
-    return best;
-}
-int env_int(const char *name, int dflt) { const char *s = std::getenv(name); return s ? std::atoi(s) : dflt; }
-int ssm_fwd_cw(const fms_ssm_args *a) { if (int v = env_int("X_FCW", 0)) return v; return best_cw(a, fms::kSsmFwdWarps, 8, 3, 1.5, ssm_fwd_smem); }
-int ssm_bwd_cw(const fms_ssm_args *a) { if (int v = env_int("X_BCW", 0)) return v; return best_cw(a, fms::kSsmBwdWarps, 8, 1, 1.5, ssm_bwd_smem); }
 
 template <typename Kernel>
 int allow_smem(Kernel kernel, size_t bytes) {
@@ -109,71 +144,93 @@ int allow_smem(Kernel kernel, size_t bytes) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
-// out[i] = sum over `count` slices of `stride` floats, in order
-__global__ void sum_slices_kernel(const float *__restrict__ part, float *__restrict__ out, int64_t n, int64_t count,
-                                  int64_t stride) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    float v = 0.f;
-    for (int64_t k = 0; k < count; ++k) v += part[k * stride + i];
-    out[i] = v;
-}
-int sum_slices(const float *part, float *out, int64_t n, int64_t count, int64_t stride, cudaStream_t st) {
-    if (!out || n == 0) return FMS_OK;
-    if ((n + 127) / 128 > kMaxGrid) return FMS_ERR_TOO_LARGE;
-    sum_slices_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, st>>>(part, out, n, count, stride);
+// The first pass over pieces of time and the fold of what they leave; REVERSE for the adjoint.
+// `carries`: (batch, segs, D, N), then the sums of time steps (batch, segs, D).
+template <typename S, bool ALIGNED, bool REVERSE>
+int launch_ssm_carries(const fms_ssm_args *a, const SsmCut &main, int warps, const S *grad_out, const float *first,
+                       float *carries, float *sums, cudaStream_t st) {
+    SsmCut cut = main;
+    cut.cw = std::min(4, std::max(1, main.cw * warps / fms::kSsmFwdWarps / 2));
+    while (cut.cw > 1 && ssm_carry_smem(a, cut.cw) > kMaxSmem) --cut.cw;
+    const auto p = ssm_problem<S>(a, cut, fms::kSsmFwdWarps);
+    const int64_t grid = p.batch * p.groups * p.chunks * p.segs, states = p.batch * p.channels * p.N;
+    if (grid > kMaxGrid || (states + 127) / 128 > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    const size_t smem = ssm_carry_smem(a, cut.cw);
+    if (int rc = allow_smem(fms::ssm_carry_kernel<S, ALIGNED, REVERSE>, smem)) return rc;
+    fms::ssm_carry_kernel<S, ALIGNED, REVERSE><<<static_cast<unsigned>(grid), fms::kSsmFwdWarps * 32, smem, st>>>(
+        p, grad_out, carries, sums);
+    if (int rc = check_launch()) return rc;
+    fms::ssm_fold_kernel<<<static_cast<unsigned>((states + 127) / 128), 128, 0, st>>>(
+        carries, sums, p.A, first, p.batch, p.channels, p.N, p.segs, REVERSE);
     return check_launch();
 }
 
+size_t carry_floats(const fms_ssm_args *a, const SsmCut &cut) {  // of the states; the sums follow
+    return cut.segs > 1 ? static_cast<size_t>(a->batch) * cut.segs * a->channels * a->states : 0;
+}
+size_t carry_bytes(const fms_ssm_args *a, const SsmCut &cut) {
+    return cut.segs > 1 ? round256(sizeof(float) * (carry_floats(a, cut) + static_cast<size_t>(a->batch) * cut.segs * a->channels)) : 0;
+}
+
 template <typename S, bool ALIGNED>
-int launch_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *ck, cudaStream_t st) {
-    const auto p = ssm_problem<S>(a, ssm_fwd_cw(a), fms::kSsmFwdWarps);
-    const int64_t grid = p.batch * p.groups * p.chunks;
+int launch_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *ck, float *ws, cudaStream_t st) {
+    const SsmCut cut = ssm_fwd_cut(a);
+    if (cut.segs > 1)
+        if (int rc = launch_ssm_carries<S, ALIGNED, false>(a, cut, fms::kSsmFwdWarps, nullptr, a->h0, ws, ws + carry_floats(a, cut), st))
+            return rc;
+    const auto p = ssm_problem<S>(a, cut, fms::kSsmFwdWarps);
+    const int64_t grid = p.batch * p.groups * p.chunks * p.segs;
     if (grid > kMaxGrid) return FMS_ERR_TOO_LARGE;
     const size_t smem = ssm_fwd_smem(a, p.cw);
     if (int rc = allow_smem(fms::ssm_forward_kernel<S, ALIGNED>, smem)) return rc;
     fms::ssm_forward_kernel<S, ALIGNED><<<static_cast<unsigned>(grid), fms::kSsmFwdWarps * 32, smem, st>>>(
-        p, static_cast<S *>(out), h_last, ck);
+        p, cut.segs > 1 ? ws : nullptr, static_cast<S *>(out), h_last, ck);
     return check_launch();
 }
 
 struct SsmScratch {
-    size_t bc, a, d, total;
+    size_t bc, a, d, carries, total;
 };
-SsmScratch ssm_scratch(const fms_ssm_args *a) {
-    const int64_t cw = ssm_bwd_cw(a), per = a->channels / a->groups;
-    const int64_t chunks = (per + cw * fms::kSsmBwdWarps - 1) / (cw * fms::kSsmBwdWarps);
+SsmScratch ssm_scratch(const fms_ssm_args *a, const SsmCut &cut) {
+    const int64_t per = a->channels / a->groups, chunks = (per + cut.cw * fms::kSsmBwdWarps - 1) / (cut.cw * fms::kSsmBwdWarps);
     const int64_t Tpad = (a->T + fms::kSsmTile - 1) / fms::kSsmTile * fms::kSsmTile;
     SsmScratch s;
     s.bc = round256(sizeof(float) * a->batch * a->groups * chunks * 2 * a->states * Tpad);
-    s.a = round256(sizeof(float) * a->batch * a->channels * a->states);
-    s.d = round256(sizeof(float) * a->batch * a->channels * 2);
-    s.total = s.bc + s.a + s.d;
+    s.a = round256(sizeof(float) * a->batch * cut.segs * a->channels * a->states);
+    s.d = round256(sizeof(float) * a->batch * cut.segs * a->channels * 2);
+    s.carries = carry_bytes(a, cut);
+    s.total = s.bc + s.a + s.d + s.carries;
     return s;
 }
 
 template <typename S, bool ALIGNED>
 int launch_ssm_backward(const fms_ssm_args *a, fms::SsmGrads<S> o, S *dB, S *dC, float *dA, float *dD, float *dbias,
                         char *ws, cudaStream_t st) {
-    const auto p = ssm_problem<S>(a, ssm_bwd_cw(a), fms::kSsmBwdWarps);
-    const SsmScratch sc = ssm_scratch(a);
+    const SsmCut cut = ssm_bwd_cut(a);
+    const auto p = ssm_problem<S>(a, cut, fms::kSsmBwdWarps);
+    const SsmScratch sc = ssm_scratch(a, cut);
     o.bc_part = reinterpret_cast<float *>(ws);
     o.a_part = reinterpret_cast<float *>(ws + sc.bc);
     o.d_part = reinterpret_cast<float *>(ws + sc.bc + sc.a);
-    const int64_t grid = p.batch * p.groups * p.chunks, rows = p.batch * p.groups * 2 * p.N;
-    if (grid > kMaxGrid || rows > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    const int64_t row_blocks = (p.T + 255) / 256, bc_blocks = p.batch * p.groups * 2 * p.N * row_blocks;
+    const int64_t finish = bc_blocks + (p.channels * (p.N + 2) + 255) / 256;
+    const int64_t grid = p.batch * p.groups * p.chunks * p.segs;
+    if (grid > kMaxGrid || finish > kMaxGrid) return FMS_ERR_TOO_LARGE;
+    if (cut.segs > 1) {
+        float *carries = reinterpret_cast<float *>(ws + sc.bc + sc.a + sc.d);
+        if (int rc = launch_ssm_carries<S, ALIGNED, true>(a, cut, fms::kSsmBwdWarps, o.grad_out, o.grad_last, carries,
+                                                          carries + carry_floats(a, cut), st))
+            return rc;
+        o.carries = carries;
+    }
     const size_t smem = ssm_bwd_smem(a, p.cw);
     auto kernel = p.z ? fms::ssm_backward_kernel<S, ALIGNED, true> : fms::ssm_backward_kernel<S, ALIGNED, false>;
     if (int rc = allow_smem(kernel, smem)) return rc;
     kernel<<<static_cast<unsigned>(grid), fms::kSsmBwdWarps * 32, smem, st>>>(p, o);
     if (int rc = check_launch()) return rc;
-    const int Tpad = p.tiles * fms::kSsmTile;
-    const dim3 g2(static_cast<unsigned>(rows), static_cast<unsigned>(std::min((p.T + 255) / 256, 65535)));
-    fms::ssm_bc_kernel<S><<<g2, 256, 0, st>>>(o.bc_part, dB, dC, p.groups, p.chunks, p.N, p.T, Tpad);
-    if (int rc = check_launch()) return rc;
-    if (int rc = sum_slices(o.a_part, dA, p.channels * p.N, p.batch, p.channels * p.N, st)) return rc;
-    if (int rc = sum_slices(o.d_part, dD, p.channels, p.batch, 2 * p.channels, st)) return rc;
-    return sum_slices(o.d_part + p.channels, dbias, p.channels, p.batch, 2 * p.channels, st);
+    fms::ssm_finish_kernel<S><<<static_cast<unsigned>(finish), 256, 0, st>>>(p, o, dB, dC, dA, dD, dbias, static_cast<unsigned>(bc_blocks),
+                                                                            static_cast<int>(row_blocks));
+    return check_launch();
 }
 
 template <typename S, bool VEC, int U>
@@ -188,7 +245,7 @@ int launch_ssm_step_u(const fms::SsmProblem<S> &p, float *state, int64_t pool, c
 }
 template <typename S>
 int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
-    const auto p = ssm_problem<S>(a, 1, 1);
+    const auto p = ssm_problem<S>(a, SsmCut{1, 1, 1}, 1);
     if (p.groups > 65535) return FMS_ERR_TOO_LARGE;
     int log_L = 0;
     while (log_L < 5 && (8 << log_L) < p.N) ++log_L;
@@ -203,9 +260,9 @@ int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int
 
 namespace {
 template <typename S>
-int ssm_forward_t(const fms_ssm_args *a, void *out, float *h_last, float *ck, cudaStream_t st) {
-    return ssm_aligned(a) && aligned_to(out, 16) ? launch_ssm_forward<S, true>(a, out, h_last, ck, st)
-                                                 : launch_ssm_forward<S, false>(a, out, h_last, ck, st);
+int ssm_forward_t(const fms_ssm_args *a, void *out, float *h_last, float *ck, float *ws, cudaStream_t st) {
+    return ssm_aligned(a) && aligned_to(out, 16) ? launch_ssm_forward<S, true>(a, out, h_last, ck, ws, st)
+                                                 : launch_ssm_forward<S, false>(a, out, h_last, ck, ws, st);
 }
 }  // namespace
 
@@ -214,7 +271,13 @@ FMS_EXPORT size_t fms_ssm_checkpoint_bytes(const fms_ssm_args *a) {
     return sizeof(float) * a->batch * a->channels * a->states * ((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
 }
 
-FMS_EXPORT int fms_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *checkpoints, fms_stream_t stream) {
+FMS_EXPORT size_t fms_ssm_forward_workspace_bytes(const fms_ssm_args *a) {
+    if (ssm_check(a) != FMS_OK || ssm_empty(a) || a->T == 0) return 0;
+    return carry_bytes(a, ssm_fwd_cut(a));
+}
+
+FMS_EXPORT int fms_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, float *checkpoints, void *workspace,
+                               size_t workspace_bytes, fms_stream_t stream) {
     if (int rc = ssm_check(a)) return rc;
     if (ssm_empty(a)) return FMS_OK;
     if (int rc = ssm_pointers(a, a->T > 0)) return rc;
@@ -222,12 +285,14 @@ FMS_EXPORT int fms_ssm_forward(const fms_ssm_args *a, void *out, float *h_last, 
     if (!aligned_to(out, elem_size(a->dtype)) || !aligned_to(h_last, 4) || !aligned_to(checkpoints, 4)) return FMS_ERR_MISALIGNED;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a->T == 0) return copy_or_zero(a->h0, h_last, a->batch * a->channels * a->states, st);
-    FMS_BY_TYPE(a->dtype, (ssm_forward_t<S>(a, out, h_last, checkpoints, st)));
+    const size_t need = fms_ssm_forward_workspace_bytes(a);
+    if (need && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < need)) return FMS_ERR_WORKSPACE;
+    FMS_BY_TYPE(a->dtype, (ssm_forward_t<S>(a, out, h_last, checkpoints, static_cast<float *>(workspace), st)));
 }
 
 FMS_EXPORT size_t fms_ssm_backward_workspace_bytes(const fms_ssm_args *a) {
     if (ssm_check(a) != FMS_OK || ssm_empty(a) || a->T == 0) return 0;
-    return ssm_scratch(a).total;
+    return ssm_scratch(a, ssm_bwd_cut(a)).total;
 }
 
 FMS_EXPORT int fms_ssm_backward(const fms_ssm_args *a, const float *checkpoints, const void *grad_out,

@@ -7,8 +7,9 @@
 // grid of 8 time lanes x 4 state lanes; a lane holds 8 consecutive positions of 4 states, so the 16
 // states of a block and the 64 positions of a tile are spread over the warp, and B and C of the tile
 // stay in registers while the warp goes through its channels.  Per channel and state a lane
-//   1. forms its 8 decays (one exponential each) and its aggregate (P, S): P the product of the decays,
-//      S the state of its positions from a zero start,
+//   1. forms its 8 decays (one exponential each) and its aggregate (P, S): P = exp(A * sum dt), one more
+//      exponential, which unlike the product of the decays does not add up their roundings over a long
+//      memory; S the state of its positions from a zero start,
 //   2. takes part in a 3-step shuffle scan of the pairs over the 8 time lanes, seeded with the carry,
 //   3. runs its 8 positions again from the state that enters them, in registers.
 // Each decay is thus computed once and the sequence is parallel over positions, channels and states;
@@ -35,6 +36,7 @@ constexpr int kSsmTile = kSsmE * kSsmTimeLanes;  // positions of a tile
 constexpr int kSsmNL = 4;                      // states of a lane
 constexpr int kSsmNB = 16;                     // states of a block (4 lanes x 4)
 constexpr int kSsmFwdWarps = 4;
+constexpr int kSsmStages = 2;                  // tiles in shared memory; three and four were no faster
 constexpr int kSsmBwdWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -52,6 +54,7 @@ struct SsmProblem {
     int chunks;         // CTAs along the channels of a group
     int tiles;
     int softplus;
+    int segs, seg_tiles;  // time is cut into segs pieces of seg_tiles tiles, each with CTAs of its own
 };
 
 // ------------------------------------------------------------------------------ arithmetic ----
@@ -92,17 +95,23 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
     return r;
 }
 
-// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) in (0, 1].  log1p(e) = 2 artanh(r) with
-// r = e / (2 + e) <= 1/3, so small e keep their relative precision; artanh(r) / r is a polynomial of degree
-// 4 in r^2, fitted at Chebyshev points of [0, 1/9] and off by at most 8e-9.  sigmoid_f is its derivative.
+// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) in (0, 1].  The argument |v| log2(e) is taken to
+// twice the precision (its rounding would cost e up to |v| roundings, and a state adds up the time steps of
+// its whole memory).  log1p(e) = 2 artanh(r) with r = e / (2 + e) <= 1/3, so small e keep their relative
+// precision; artanh(r) / r is a polynomial of degree 4 in r^2, fitted at Chebyshev points of [0, 1/9] and off
+// by at most 8e-9.  sigmoid_f is its derivative.
 __device__ __forceinline__ float softplus_f(float v) {
-    const float e = ex2(-kLog2e * fabsf(v));
+    constexpr float kLog2eLow = 1.925963033500e-8f, kLn2f = 0.6931471805599453f;  // log2(e) - kLog2e
+    const float w = -fabsf(v), t = w * kLog2e, low = fmaf(w, kLog2e, -t) + w * kLog2eLow;
+    float e = ex2(t);
+    e = fmaf(e, low * kLn2f, e);
     const float r = e * rcp(2.f + e), q = r * r;
     float s = fmaf(0.14087329f, q, 0.13980709f);
     s = fmaf(s, q, 0.20012427f);
     s = fmaf(s, q, 0.33333158f);
     s = fmaf(s, q, 1.f);
-    return fmaf(r + r, s, v > 0.f ? v : v != v ? v : 0.f);
+    const float y = fmaf(r + r, s, v > 0.f ? v : v != v ? v : 0.f);
+    return w < -80.f ? fmaxf(v, 0.f) : y;  // beyond, e is not a normal number and its correction no number
 }
 
 template <typename S>
@@ -135,8 +144,13 @@ __host__ __device__ constexpr int row_bytes() { return kSsmTile * static_cast<in
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// All of this thread's copies but those of the N newest groups have arrived.
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Thread `i` of `n` (a multiple of 32) copies its granules of `rows` rows; src(row) gives a row's first
 // position (t = 0), or null for a row of zeros.  `any`: some valid address, named by copies that read nothing.
@@ -336,20 +350,20 @@ __device__ __forceinline__ f2 lane_scan2(f2 P, f2 &S, f2 carry, int s) {
     const f2 in = lane_move<UP>(S, 1);
     return r == 0 ? carry : in;
 }
-__device__ __forceinline__ float product8(const f2 (&a)[4]) {
-    const f2 m = mul2(mul2(a[0], a[1]), mul2(a[2], a[3]));
-    return lo(m) * hi(m);
-}
-
 // Which channels a warp has: [c0, c0 + nc) of group g of sequence b; nc may be <= 0.
 struct SsmPlace {
     int64_t b, d0;  // sequence; first channel counted over all groups
     int g, chunk, nc;
+    int seg, first, last;  // piece of time: tiles [first, last)
 };
 template <typename S>
 __device__ __forceinline__ SsmPlace ssm_place(const SsmProblem<S> &p, int warps) {
     SsmPlace w;
     int64_t k = blockIdx.x;
+    w.seg = static_cast<int>(k % p.segs);
+    k /= p.segs;
+    w.first = w.seg * p.seg_tiles;
+    w.last = min(p.tiles, w.first + p.seg_tiles);
     w.chunk = static_cast<int>(k % p.chunks);
     k /= p.chunks;
     w.g = static_cast<int>(k % p.groups);
@@ -418,22 +432,35 @@ __device__ __forceinline__ void states_out(float *__restrict__ to, const float *
     }
 }
 
-// bytes of shared memory: forward per CTA and warp; backward likewise
+// bytes of shared memory: B and C of a CTA; the rest of a warp, forward and backward
 template <typename S>
-inline __host__ __device__ size_t ssm_bc_bytes() { return 2 * 2 * kSsmNB * row_bytes<S>(); }
+inline __host__ __device__ size_t ssm_bc_bytes() { return kSsmStages * 2 * kSsmNB * row_bytes<S>(); }
 template <typename S>
 inline __host__ __device__ size_t ssm_fwd_warp_bytes(int cw, int NP) {
     return cw * (2 * 3 * row_bytes<S>() + sizeof(float) * (3 * kSsmTile + 2 * NP + 4));
 }
 template <typename S>
 inline __host__ __device__ size_t ssm_bwd_warp_bytes(int cw, int NP) {
-    return cw * (2 * 4 * row_bytes<S>() + sizeof(float) * (6 * kSsmTile + 4 * NP + 36));
+    return cw * (kSsmStages * (4 * row_bytes<S>() + sizeof(float) * NP) + sizeof(float) * (6 * kSsmTile + 3 * NP + 36));
 }
+
+// Position in the walk of (tile, block of states) steps, and the places of its copies in their rings.
+struct SsmWalk {
+    int tile, nb, slot, row_slot;
+    __device__ __forceinline__ void next(int blocks, int dir) {
+        slot ^= 1;
+        if (++nb == blocks) {
+            nb = 0;
+            tile += dir;
+            row_slot ^= 1;
+        }
+    }
+};
 
 template <typename S, bool ALIGNED>
 __global__ void __launch_bounds__(kSsmFwdWarps * 32, 3)
-ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict__ h_last,
-                   float *__restrict__ checkpoints) {
+ssm_forward_kernel(const SsmProblem<S> p, const float *__restrict__ carries, S *__restrict__ out,
+                   float *__restrict__ h_last, float *__restrict__ checkpoints) {
     extern __shared__ __align__(16) unsigned char ssm_smem[];
     constexpr int RB = row_bytes<S>();
     const int lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3;
@@ -451,14 +478,17 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
     for (int c = 0; c < w.nc; ++c)
         for (int n = lane; n < p.NP; n += 32) {
             A_[c * p.NP + n] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
-            h_[c * p.NP + n] = n < p.N && p.h0 ? p.h0[(row0 + c) * p.N + n] : 0.f;
+            // a piece of time starts from the state that the pieces before it leave
+            const float *h0 = carries ? carries + ((w.b * p.segs + w.seg) * p.channels + w.d0) * p.N
+                                      : p.h0 ? p.h0 + row0 * p.N : nullptr;
+            h_[c * p.NP + n] = n < p.N && h0 ? h0[c * p.N + n] : 0.f;
         }
     if (lane < w.nc) {  // at most 8 channels
         bias_[lane] = p.bias ? p.bias[w.d0 + lane] : 0.f;
         D_[lane] = p.D ? p.D[w.d0 + lane] : 0.f;
     }
 
-    const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
+    const int blocks = p.NP / kSsmNB, live_tiles = min(w.last, (len + kSsmTile - 1) / kSsmTile);
     const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
     const S *xw = whole_src(xrow, p.xs[1], lane), *dw = whole_src(drow, p.ds[1], lane);
     const S *zw = p.z ? whole_src(zrow, p.zs[1], lane) : nullptr;
@@ -490,16 +520,17 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
             });
         copies_commit();
     };
-    if (live_tiles > 0) stage(0, 0, 0);
+    if (live_tiles > w.first) stage(w.first, 0, 0);
 
-    for (int tile = 0, step = 0; tile < live_tiles; ++tile) {
+    for (int tile = w.first, step = 0; tile < live_tiles; ++tile) {
         const int g = lane & 15, t = tile * kSsmTile + 4 * g;  // outside the state loop a lane has four positions of a channel
         const unsigned char *mine = raw + (tile & 1) * (3 * p.cw * RB);
         for (int nb = 0; nb < blocks; ++nb, ++step) {
-            copies_wait();
+            copies_wait<0>();
             __syncthreads();
             if (nb + 1 < blocks) stage(tile, nb + 1, step + 1);
             else if (tile + 1 < live_tiles) stage(tile + 1, 0, step + 1);
+            const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
             if (nb == 0) {
                 for (int c = lane >> 4; c < w.nc; c += 2) {
                     float x[4], dt[4];
@@ -518,7 +549,6 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
             const int n0 = nb * kSsmNB + q * kSsmNL;
             f2 B[2][8], C[2][8];  // [pair of states][position]
             {
-                const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int r = q * kSsmNL + 2 * j, n = n0 + 2 * j;
@@ -535,6 +565,7 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
                 f2 dt[8], u[8], y[8];
                 tile_get_twice(dt_ + c * kSsmTile, s, dt);
                 tile_get_twice(u_ + c * kSsmTile, s, u);
+                const f2 span = add2(add2(add2(dt[0], dt[1]), add2(dt[2], dt[3])), add2(add2(dt[4], dt[5]), add2(dt[6], dt[7])));
                 const float4 A4 = *reinterpret_cast<const float4 *>(A_ + c * p.NP + n0);
                 const float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
                 __syncwarp();  // the carries are read before the last time lane replaces them
@@ -549,12 +580,10 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
                         a[i] = pk(ex2(lo(e)), ex2(hi(e)));
                         b[i] = mul2(u[i], B[j][i]);
                     }
-                    f2 S0 = b[0], P = a[0];
+                    const f2 e = mul2(span, Av[j]), P = pk(ex2(lo(e)), ex2(hi(e)));
+                    f2 S0 = b[0];
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) {
-                        S0 = fma2(a[i], S0, b[i]);
-                        P = mul2(P, a[i]);
-                    }
+                    for (int i = 1; i < 8; ++i) S0 = fma2(a[i], S0, b[i]);
                     f2 h = lane_scan2<true>(P, S0, hv[j], s);
                     hv[j] = S0;
 #pragma unroll
@@ -591,10 +620,10 @@ ssm_forward_kernel(const SsmProblem<S> p, S *__restrict__ out, float *__restrict
     }
     __syncwarp();
     const float zero[4] = {};
-    for (int tile = live_tiles; tile < p.tiles; ++tile)  // behind the sequence: zeros
+    for (int tile = max(w.first, live_tiles); tile < w.last; ++tile)  // behind the sequence: zeros
         for (int c = lane >> 4; c < w.nc; c += 2)
             store_four<S, ALIGNED>(out + (row0 + c) * p.T, tile * kSsmTile + 4 * (lane & 15), p.T, zero);
-    if (h_last && w.nc > 0) states_out(h_last + row0 * p.N, h_, w.nc, p.N, p.NP, lane);
+    if (h_last && w.nc > 0 && w.seg == p.segs - 1) states_out(h_last + row0 * p.N, h_, w.nc, p.N, p.NP, lane);
 }
 
 // What the backward writes; the partial sums live in the caller's workspace.
@@ -602,12 +631,12 @@ template <typename S>
 struct SsmGrads {
     const float *checkpoints;
     const S *grad_out;
-    const float *grad_last;
+    const float *grad_last, *carries;
     S *dx, *ddelta, *dz;
     float *dh0;
     float *bc_part;  // [batch][group][chunk][B | C][N][tiles * 64]
-    float *a_part;   // [batch][D][N]
-    float *d_part;   // [batch][2][D]: grad of D, grad of delta_bias
+    float *a_part;   // [batch][segment][D][N]
+    float *d_part;   // [batch][segment][2][D]: grad of D, grad of delta_bias
 };
 
 // With e_t = C_t dy_t:  c_t = a_t (e_t + c_{t+1}) is what reaches the state before t, g_t = e_t + c_{t+1},
@@ -629,9 +658,9 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
     float *red = reinterpret_cast<float *>(ssm_smem + ssm_bc_bytes<S>());  // [warp][64][lane]
     unsigned char *raw = reinterpret_cast<unsigned char *>(red + W * 64 * 32) + warp * ssm_bwd_warp_bytes<S>(p.cw, p.NP);
     const int ct = p.cw * kSsmTile, cn = p.cw * p.NP;
-    float *dt_ = reinterpret_cast<float *>(raw + 2 * 4 * p.cw * RB);
+    float *ck_ = reinterpret_cast<float *>(raw + kSsmStages * 4 * p.cw * RB), *dt_ = ck_ + kSsmStages * cn;
     float *u_ = dt_ + ct, *dy_ = u_ + ct, *gB_ = dy_ + ct, *q_ = gB_ + ct, *y_ = q_ + ct;
-    float *A_ = y_ + ct, *h_ = A_ + cn, *c_ = h_ + cn, *dA_ = c_ + cn, *dD_ = dA_ + cn, *bias_ = dD_ + 32 * p.cw, *D_ = bias_ + p.cw;
+    float *A_ = y_ + ct, *c_ = A_ + cn, *dA_ = c_ + cn, *dD_ = dA_ + cn, *bias_ = dD_ + 32 * p.cw, *D_ = bias_ + p.cw;
     const int len = ssm_length(p, w.b);
     const int64_t row0 = w.b * p.channels + w.d0;
     const int Tpad = p.tiles * kSsmTile;
@@ -644,8 +673,10 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
         for (int n = lane; n < p.NP; n += 32) {
             const int i = c * p.NP + n;
             A_[i] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
-            c_[i] = n < p.N && o.grad_last ? o.grad_last[(row0 + c) * p.N + n] : 0.f;
-            h_[i] = 0.f;
+            const float *c0 = o.carries ? o.carries + ((w.b * p.segs + w.seg) * p.channels + w.d0) * p.N
+                                        : o.grad_last ? o.grad_last + row0 * p.N : nullptr;
+            c_[i] = n < p.N && c0 ? c0[c * p.N + n] : 0.f;
+            for (int k = 0; k < kSsmStages; ++k) ck_[k * cn + i] = 0.f;
             dA_[i] = 0.f;
         }
         dD_[c * 32 + lane] = 0.f;
@@ -655,15 +686,31 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
         }
     }
 
-    const int blocks = p.NP / kSsmNB, live_tiles = (len + kSsmTile - 1) / kSsmTile;
+    const int blocks = p.NP / kSsmNB, live_tiles = min(w.last, (len + kSsmTile - 1) / kSsmTile);
     const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
     const int64_t T = p.T;
     const S *xw = whole_src(xrow, p.xs[1], lane), *dw = whole_src(drow, p.ds[1], lane), *gw = whole_src(grow, T, lane);
     const S *zw = GATED ? whole_src(zrow, p.zs[1], lane) : nullptr;
     const S *Bw = whole_src(Brow, p.Bs[2], threadIdx.x), *Cw = whole_src(Crow, p.Cs[2], threadIdx.x);
-    auto stage = [&](int tile, int nb, int step) {
-        const int t0 = tile * kSsmTile;
-        unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB), *to = raw + (tile & 1) * (4 * p.cw * RB);
+    SsmWalk ahead{live_tiles - 1, 0, 0, 0}, at = ahead;
+    const bool ck_whole = p.N == p.NP && (reinterpret_cast<uintptr_t>(o.checkpoints) & 15) == 0;
+    auto stage = [&]() {  // the copies of the next step; past the end an empty group, which keeps the count
+        if (ahead.tile < w.first) {
+            copies_commit();
+            return;
+        }
+        const int nb = ahead.nb, t0 = ahead.tile * kSsmTile;
+        unsigned char *bc = ssm_smem + ahead.slot * (2 * kSsmNB * RB), *to = raw + ahead.row_slot * (4 * p.cw * RB);
+        if (nb == 0) {  // the states in front of the tile
+            const float *ck = o.checkpoints + ((w.b * p.tiles + ahead.tile) * p.channels + w.d0) * p.N;
+            const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ck_ + ahead.row_slot * cn));
+            if (ck_whole) {
+                for (int i = lane; i < w.nc * p.N / 4; i += 32) copy16(dst + i * 16, ck + i * 4, 16);
+            } else {
+                for (int c = 0; c < w.nc; ++c)
+                    for (int n = lane; n < p.N; n += 32) copy4(dst + (c * p.NP + n) * 4, ck + c * p.N + n);
+            }
+        }
         if (ALIGNED && t0 + kSsmTile <= len) {
             constexpr int n = W * 32;
             if ((nb + 1) * kSsmNB <= p.N) {
@@ -689,6 +736,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                 return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
             });
         copies_commit();
+        ahead.next(blocks, -1);
     };
     const int g4 = lane & 15;  // outside the state loop a lane has four positions of a channel
     auto row_at = [&](const unsigned char *mine, int kind, int c, float (&f)[4]) {
@@ -699,7 +747,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
         row_four<S, ALIGNED>(mine + (kind * p.cw + c) * RB, row_shift<S, ALIGNED>(first), g4, f);
     };
 
-    for (int tile = p.tiles - 1; tile >= live_tiles; --tile) {  // behind the sequence: zeros
+    for (int tile = max(w.first, live_tiles); tile < w.last; ++tile) {  // behind the sequence: zeros
         const int t = tile * kSsmTile + 4 * g4;
         const float zero[4] = {};
         for (int c = lane >> 4; c < w.nc; c += 2) {
@@ -710,20 +758,20 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
         for (int i = threadIdx.x; i < 2 * p.N * kSsmTile; i += W * 32)
             bc_out[static_cast<int64_t>(i / kSsmTile) * Tpad + tile * kSsmTile + i % kSsmTile] = 0.f;
     }
-    if (live_tiles > 0) stage(live_tiles - 1, 0, 0);
+    __syncwarp();  // the states' places are cleared
+    for (int k = 1; k < kSsmStages; ++k) stage();
 
-    for (int tile = live_tiles - 1, step = 0; tile >= 0; --tile) {
+    for (int tile = live_tiles - 1; tile >= w.first; --tile) {
         const int t = tile * kSsmTile + 4 * g4;
-        const unsigned char *mine = raw + (tile & 1) * (4 * p.cw * RB);
-        for (int nb = 0; nb < blocks; ++nb, ++step) {
-            copies_wait();
+        const unsigned char *mine = raw + at.row_slot * (4 * p.cw * RB);
+        const float *h_ = ck_ + at.row_slot * cn;
+        for (int nb = 0; nb < blocks; ++nb) {
+            copies_wait<0>();
             __syncthreads();
-            if (nb + 1 < blocks) stage(tile, nb + 1, step + 1);
-            else if (tile > 0) stage(tile - 1, 0, step + 1);
+            stage();
+            const unsigned char *bc = ssm_smem + at.slot * (2 * kSsmNB * RB);
+            at.next(blocks, -1);
             if (nb == 0) {
-                const float *ck = o.checkpoints + ((w.b * p.tiles + tile) * p.channels + w.d0) * p.N;
-                for (int c = 0; c < w.nc; ++c)
-                    for (int n = lane; n < p.N; n += 32) h_[c * p.NP + n] = ck[c * p.N + n];
                 for (int c = lane >> 4; c < w.nc; c += 2) {
                     float x[4], dt[4], dy[4];
                     row_at(mine, 0, c, x);
@@ -747,7 +795,6 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             const int n0 = nb * kSsmNB + q * kSsmNL;
             f2 B[kSsmNL][4], C[kSsmNL][4], dB[kSsmNL][4], dC[kSsmNL][4];
             {
-                const unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB);
 #pragma unroll
                 for (int j = 0; j < kSsmNL; ++j) {
                     const int r = q * kSsmNL + j;
@@ -763,6 +810,8 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                 tile_get(dt_ + c * kSsmTile, s, dt);
                 tile_get(u_ + c * kSsmTile, s, u);
                 tile_get(dy_ + c * kSsmTile, s, dy);
+                const f2 both = add2(add2(dt[0], dt[1]), add2(dt[2], dt[3]));
+                const float sum = lo(both) + hi(both);
                 const int at = c * p.NP + n0;
                 const float4 A4 = *reinterpret_cast<const float4 *>(A_ + at), h4 = *reinterpret_cast<const float4 *>(h_ + at);
                 const float4 c4 = *reinterpret_cast<const float4 *>(c_ + at);
@@ -787,7 +836,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                         if (k) S0 = fmaf(lo(a[k]), S0, lo(v[k]));
                         S0 = fmaf(hi(a[k]), S0, hi(v[k]));
                     }
-                    const float P = product8(a);
+                    const float P = ex2(sum * Av[j]);
                     const float hin = lane_scan<true>(P, S0, hv[j], s);
                     f2 h[4], e[4];
 #pragma unroll
@@ -909,35 +958,231 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
         }
     }
     __syncwarp();
+    const int64_t part = w.b * p.segs + w.seg;
     for (int c = 0; c < w.nc; ++c) {
         for (int n = lane; n < p.N; n += 32) {
             const int k = c * p.NP + n;
-            o.a_part[(row0 + c) * p.N + n] = dA_[k];
-            if (o.dh0) o.dh0[(row0 + c) * p.N + n] = c_[k];
+            o.a_part[(part * p.channels + w.d0 + c) * p.N + n] = dA_[k];
+            if (o.dh0 && w.seg == 0) o.dh0[(row0 + c) * p.N + n] = c_[k];
         }
         if (lane < 2) {  // grad D, grad delta_bias: the 16 lanes' shares in order
             float v = 0.f;
             for (int i = 0; i < 16; ++i) v += dD_[(c * 16 + i) * 2 + lane];
-            o.d_part[(w.b * 2 + lane) * p.channels + w.d0 + c] = v;
+            o.d_part[(part * 2 + lane) * p.channels + w.d0 + c] = v;
         }
     }
 }
 
-// grad_B, grad_C: the chunks' partial sums in order, rounded once.
+// First pass over a time that is cut into pieces: what each piece leaves to the next from a zero start.
+// Forward the state h at its end, REVERSE the adjoint c at its beginning; with both the sum of its time
+// steps, whose exponential is the piece's product of decays.  The second pass is the kernels above.
 template <typename S>
-__global__ void ssm_bc_kernel(const float *__restrict__ part, S *__restrict__ dB, S *__restrict__ dC, int64_t groups,
-                              int chunks, int N, int T, int Tpad) {
-    const int64_t row = blockIdx.x;  // (batch * group, which, n)
-    const int n = static_cast<int>(row % N), which = static_cast<int>(row / N % 2);
-    const int64_t bg = row / N / 2;
-    const float *src = part + ((bg * chunks) * 2 + which) * N * static_cast<int64_t>(Tpad) + n * static_cast<int64_t>(Tpad);
-    S *dst = (which ? dC : dB) + (bg * N + n) * T;
-    const int64_t step = 2 * static_cast<int64_t>(N) * Tpad;
-    for (int t = blockIdx.y * blockDim.x + threadIdx.x; t < T; t += gridDim.y * blockDim.x) {
-        float v = 0.f;
-        for (int k = 0; k < chunks; ++k) v += src[k * step + t];
-        dst[t] = from_float<S>(v);
+inline __host__ __device__ size_t ssm_carry_warp_bytes(int cw, int NP) {
+    return cw * (kSsmStages * 3 * row_bytes<S>() + sizeof(float) * (2 * kSsmTile + 2 * NP + 20));
+}
+template <typename S, bool ALIGNED, bool REVERSE>
+__global__ void __launch_bounds__(kSsmFwdWarps * 32, 3)
+ssm_carry_kernel(const SsmProblem<S> p, const S *__restrict__ grad_out, float *__restrict__ carries,
+                 float *__restrict__ sums) {
+    extern __shared__ __align__(16) unsigned char ssm_smem[];
+    constexpr int RB = row_bytes<S>(), n_threads = kSsmFwdWarps * 32;
+    const int lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3, g = lane & 15;
+    const SsmPlace w = ssm_place(p, kSsmFwdWarps);
+    unsigned char *raw = ssm_smem + ssm_bc_bytes<S>() + (threadIdx.x >> 5) * ssm_carry_warp_bytes<S>(p.cw, p.NP);
+    float *dt_ = reinterpret_cast<float *>(raw + kSsmStages * 3 * p.cw * RB), *u_ = dt_ + p.cw * kSsmTile;  // u_: REVERSE dy
+    float *h_ = u_ + p.cw * kSsmTile, *A_ = h_ + p.cw * p.NP, *sum_ = A_ + p.cw * p.NP, *bias_ = sum_ + 16 * p.cw;
+    const int len = ssm_length(p, w.b);
+    const int64_t row0 = w.b * p.channels + w.d0, T = p.T;
+    // rows: delta; tokens, or reverse grad_out and z.  Reverse reads C, forward B.
+    const S *drow = p.delta + w.b * p.ds[0] + w.d0 * p.ds[1];
+    const S *xrow = REVERSE ? grad_out + row0 * T : p.x + w.b * p.xs[0] + w.d0 * p.xs[1];
+    const S *zrow = REVERSE && p.z ? p.z + w.b * p.zs[0] + w.d0 * p.zs[1] : nullptr;
+    const int64_t xs = REVERSE ? T : p.xs[1], vs = REVERSE ? p.Cs[2] : p.Bs[2];
+    const S *vrow = REVERSE ? p.C + w.b * p.Cs[0] + w.g * p.Cs[1] : p.B + w.b * p.Bs[0] + w.g * p.Bs[1];
+
+    for (int c = 0; c < w.nc; ++c) {
+        for (int n = lane; n < p.NP; n += 32) {
+            A_[c * p.NP + n] = n < p.N ? p.A[(w.d0 + c) * p.N + n] * kLog2e : 0.f;
+            h_[c * p.NP + n] = 0.f;
+        }
+        if (lane < 16) sum_[c * 16 + lane] = 0.f;
+        if (lane == 0) bias_[c] = p.bias ? p.bias[w.d0 + c] : 0.f;
     }
+
+    const int blocks = p.NP / kSsmNB, live_tiles = min(w.last, (len + kSsmTile - 1) / kSsmTile);
+    const void *any = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(p.x) & ~uintptr_t{15});
+    const int dir = REVERSE ? -1 : 1, end = REVERSE ? w.first - 1 : max(w.first, live_tiles);
+    SsmWalk ahead{REVERSE ? max(w.first, live_tiles) - 1 : w.first, 0, 0, 0}, at = ahead;
+    auto stage = [&]() {  // the copies of the next step; past the end an empty group, which keeps the count
+        if (ahead.tile == end) {
+            copies_commit();
+            return;
+        }
+        const int nb = ahead.nb, t0 = ahead.tile * kSsmTile;
+        unsigned char *to = raw + ahead.row_slot * (3 * p.cw * RB);
+        if (nb == 0) {
+            stage_rows<S, ALIGNED>(to, w.nc, t0, len, lane, 32, any, [&](int c) { return drow + c * p.ds[1]; });
+            stage_rows<S, ALIGNED>(to + p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return xrow + c * xs; });
+            if (zrow)
+                stage_rows<S, ALIGNED>(to + 2 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return zrow + c * p.zs[1]; });
+        }
+        stage_rows<S, ALIGNED>(ssm_smem + ahead.slot * (kSsmNB * RB), kSsmNB, t0, len, threadIdx.x, n_threads, any,
+                               [&](int r) -> const S * {
+                                   const int n = nb * kSsmNB + r;
+                                   return n < p.N ? vrow + n * vs : nullptr;
+                               });
+        copies_commit();
+        ahead.next(blocks, dir);
+    };
+    for (int k = 1; k < kSsmStages; ++k) stage();
+    while (at.tile != end) {
+        const int nb = at.nb, t = at.tile * kSsmTile + 4 * g;
+        const unsigned char *mine = raw + at.row_slot * (3 * p.cw * RB), *bc = ssm_smem + at.slot * (kSsmNB * RB);
+        copies_wait<0>();
+        __syncthreads();
+        stage();
+        at.next(blocks, dir);
+        if (nb == 0) {
+            for (int c = lane >> 4; c < w.nc; c += 2) {
+                float x[4], dt[4];
+                row_four<S, ALIGNED>(mine + c * RB, row_shift<S, ALIGNED>(drow + c * p.ds[1]), g, dt);
+                row_four<S, ALIGNED>(mine + (p.cw + c) * RB, row_shift<S, ALIGNED>(xrow + c * xs), g, x);
+                time_steps(dt, bias_[c], p.softplus, t, len);
+                if (REVERSE) {
+                    if (zrow) {
+                        float z[4];
+                        row_four<S, ALIGNED>(mine + (2 * p.cw + c) * RB, row_shift<S, ALIGNED>(zrow + c * p.zs[1]), g, z);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] *= z[k] * sigmoid_f(z[k]);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] *= dt[k];
+                }
+                tile_put(dt_ + c * kSsmTile, g, dt);
+                tile_put(u_ + c * kSsmTile, g, x);
+                sum_[c * 16 + g] += (dt[0] + dt[1]) + (dt[2] + dt[3]);
+            }
+            __syncwarp();
+        }
+        const int n0 = nb * kSsmNB + q * kSsmNL;
+        f2 V[2][8];
+        {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = q * kSsmNL + 2 * j, n = n0 + 2 * j;
+                f2 e[4], o[4];
+                row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(vrow + n * vs), s, e);
+                row_eight<S, ALIGNED>(bc + (r + 1) * RB, row_shift<S, ALIGNED>(vrow + (n + 1) * vs), s, o);
+                zip8(e, o, V[j]);
+            }
+        }
+        for (int c = 0; c < w.nc; ++c) {
+            f2 dt[8], u[8];
+            tile_get_twice(dt_ + c * kSsmTile, s, dt);
+            tile_get_twice(u_ + c * kSsmTile, s, u);
+            const f2 span = add2(add2(add2(dt[0], dt[1]), add2(dt[2], dt[3])), add2(add2(dt[4], dt[5]), add2(dt[6], dt[7])));
+            const float4 A4 = *reinterpret_cast<const float4 *>(A_ + c * p.NP + n0);
+            const float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
+            __syncwarp();
+            const f2 Av[2] = {pk(A4.x, A4.y), pk(A4.z, A4.w)};
+            f2 hv[2] = {pk(h4.x, h4.y), pk(h4.z, h4.w)};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f2 all = mul2(span, Av[j]), P = pk(ex2(lo(all)), ex2(hi(all)));
+                f2 S0 = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int i8 = REVERSE ? 7 - k : k;
+                    const f2 e = mul2(dt[i8], Av[j]), a = pk(ex2(lo(e)), ex2(hi(e))), b = mul2(u[i8], V[j][i8]);
+                    // h = a h + u B;  reverse c = a (C dy + c)
+                    S0 = REVERSE ? mul2(a, k ? add2(S0, b) : b) : (k ? fma2(a, S0, b) : b);
+                }
+                lane_scan2<!REVERSE>(P, S0, hv[j], s);
+                hv[j] = S0;
+            }
+            if (s == (REVERSE ? 0 : 7))
+                *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(lo(hv[0]), hi(hv[0]), lo(hv[1]), hi(hv[1]));
+        }
+    }
+    __syncwarp();
+    if (w.nc > 0) {
+        const int64_t row = (w.b * p.segs + w.seg) * p.channels + w.d0;
+        states_out(carries + row * p.N, h_, w.nc, p.N, p.NP, lane);
+        if (lane < w.nc) {
+            float v = 0.f;
+            for (int i = 0; i < 16; ++i) v += sum_[lane * 16 + i];
+            sums[row + lane] = v;
+        }
+    }
+}
+
+// In place: what each piece leaves becomes what enters it, in the order of the scan from `first` on.
+static __global__ void __launch_bounds__(128)
+ssm_fold_kernel(float *__restrict__ carries, const float *__restrict__ sums, const float *__restrict__ A,
+                const float *__restrict__ first, int64_t batch, int64_t channels, int N, int segs, int reverse) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, per = channels * N;
+    if (i >= batch * per) return;
+    const int64_t b = i / per, k = i - b * per, d = k / N;
+    const float a = A[k] * kLog2e;
+    float carry = first ? first[i] : 0.f;
+    constexpr int M = 8;  // loads ahead of the serial fold
+    for (int j0 = 0; j0 < segs; j0 += M) {
+        float c[M], t[M];
+#pragma unroll
+        for (int j = 0; j < M; ++j)
+            if (j0 + j < segs) {
+                const int64_t seg = b * segs + (reverse ? segs - 1 - j0 - j : j0 + j);
+                c[j] = carries[seg * per + k];
+                t[j] = sums[seg * channels + d];
+            }
+#pragma unroll
+        for (int j = 0; j < M; ++j)
+            if (j0 + j < segs) {
+                const int64_t seg = b * segs + (reverse ? segs - 1 - j0 - j : j0 + j);
+                carries[seg * per + k] = carry;
+                carry = fmaf(ex2(a * t[j]), carry, c[j]);
+            }
+    }
+}
+
+// The last sums of the backward in one launch, each in a fixed order.  Blocks below `bc_blocks`: grad_B and
+// grad_C over the CTAs along the channels, 256 positions of a row (sequence, group, B | C, state) each; the
+// others: grad_A, grad_D and grad_delta_bias over the sequences and pieces of time.
+template <typename S>
+__global__ void __launch_bounds__(256)
+ssm_finish_kernel(const SsmProblem<S> p, const SsmGrads<S> o, S *__restrict__ dB, S *__restrict__ dC, float *__restrict__ dA,
+                  float *__restrict__ dD, float *__restrict__ dbias, unsigned bc_blocks, int row_blocks) {
+    if (blockIdx.x < bc_blocks) {
+        const int Tpad = p.tiles * kSsmTile;
+        const int64_t row = blockIdx.x / row_blocks, bg = row / (2 * p.N);
+        const int r = static_cast<int>(row - bg * 2 * p.N), which = r >= p.N, n = r - which * p.N;
+        const int t = static_cast<int>(blockIdx.x - row * row_blocks) * 256 + threadIdx.x;
+        if (t >= p.T) return;
+        const int64_t step = 2 * static_cast<int64_t>(p.N) * Tpad;
+        const float *src = o.bc_part + bg * p.chunks * step + r * static_cast<int64_t>(Tpad) + t;
+        float v = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < p.chunks; ++k) v += src[k * step];
+        (which ? dC : dB)[(bg * p.N + n) * p.T + t] = from_float<S>(v);
+        return;
+    }
+    int64_t i = static_cast<int64_t>(blockIdx.x - bc_blocks) * 256 + threadIdx.x;
+    const int64_t nA = p.channels * p.N, parts = p.batch * p.segs;
+    const float *src = o.a_part;
+    int64_t step = nA;
+    float *dst = dA;
+    if (i >= nA) {
+        i -= nA;
+        if (i >= 2 * p.channels) return;
+        src = o.d_part, step = 2 * p.channels;
+        dst = i < p.channels ? dD : dbias ? dbias - p.channels : nullptr;
+        if (!dst) return;
+    }
+    float v = 0.f;
+#pragma unroll 4
+    for (int64_t k = 0; k < parts; ++k) v += src[k * step + i];
+    dst[i] = v;
 }
 
 // ---------------------------------------------------------------- one token ------------------

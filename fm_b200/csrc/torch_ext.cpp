@@ -497,8 +497,11 @@ static std::tuple<at::Tensor, OptTensor, OptTensor> ssm_forward(
     OptTensor last, ck;
     if (want_last) last = at::empty({a.batch, a.channels, a.states}, A.options());
     if (want_checkpoints) ck = at::empty({static_cast<int64_t>(fms_ssm_checkpoint_bytes(&a) / 4)}, A.options());
+    const size_t scratch = fms_ssm_forward_workspace_bytes(&a);
+    at::Tensor ws;
+    if (scratch) ws = at::empty({static_cast<int64_t>(scratch)}, x.options().dtype(at::kByte));
     check_status(fms_ssm_forward(&a, out.data_ptr(), want_last ? last->data_ptr<float>() : nullptr,
-                                 want_checkpoints ? ck->data_ptr<float>() : nullptr,
+                                 want_checkpoints ? ck->data_ptr<float>() : nullptr, scratch ? ws.data_ptr() : nullptr, scratch,
                                  at::cuda::getCurrentCUDAStream().stream()),
                  "ssm_scan");
     return {out, last, ck};

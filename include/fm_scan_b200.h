@@ -436,9 +436,13 @@ typedef struct fms_ssm_args {
 /*
  * Forward.  out (B, D, T); h_last (B, D, N) fp32, nullable; checkpoints: nullable, fp32, of
  * fms_ssm_checkpoint_bytes(), receives the states the backward starts its blocks of positions from.
+ * workspace: 16-byte aligned, fms_ssm_forward_workspace_bytes() (0 unless a few rows make it pay to cut
+ * time into pieces).
  */
 size_t fms_ssm_checkpoint_bytes(const fms_ssm_args *args);
-int fms_ssm_forward(const fms_ssm_args *args, void *out, float *h_last, float *checkpoints, fms_stream_t stream);
+size_t fms_ssm_forward_workspace_bytes(const fms_ssm_args *args);
+int fms_ssm_forward(const fms_ssm_args *args, void *out, float *h_last, float *checkpoints, void *workspace,
+                    size_t workspace_bytes, fms_stream_t stream);
 
 /*
  * Backward of the above from grad_out (B, D, T, contiguous) and grad_last (B, D, N) fp32, nullable.

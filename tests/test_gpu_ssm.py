@@ -120,6 +120,16 @@ def test_scan_and_gradients_match_the_formula(case, softplus):
     check_scan(i, grads, softplus)
 
 
+# few rows and a long time: the time is cut into pieces that are scanned side by side
+LONG = [("f32", 1, 2, 1100, 16, 1, True, True, True, True, None), ("bf16", 2, 5, 1001, 20, 1, False, True, True, True, [1001, 130]),
+        ("f16", 1, 40, 2048, 16, 2, True, True, True, False, None), ("f32", 3, 4, 1500, 3, 1, True, False, True, True, [64, 0, 1499])]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c[:6])))
+def test_scan_of_few_long_rows(case):
+    check_scan(*scan_case(*case, seed=77))
+
+
 @pytest.mark.parametrize("T", [2, 15, 16, 17, 127, 128, 130])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_scan_of_every_residue(T, dtype):

@@ -120,7 +120,7 @@ def conv_args(p, **kw):
 def test_scan_entry_refuses(change, status):
     keep, p = _p()
     a = ssm_args(p, **change)
-    assert capi.call("fms_ssm_forward", a, p, None, None, None, check=False) == status
+    assert capi.call("fms_ssm_forward", a, p, None, None, None, 0, None, check=False) == status
     if change.get("T") is None or change["T"] < 0:
         assert capi.call("fms_ssm_backward", a, p, p, None, p, p, None, p, p, p, None, None, None, p, 1 << 30, None,
                          check=False) == status
@@ -129,7 +129,7 @@ def test_scan_entry_refuses(change, status):
 def test_scan_entry_refuses_pointers_and_scratch():
     keep, p = _p()
     a = ssm_args(p)
-    fwd = lambda a, out: capi.call("fms_ssm_forward", a, out, None, None, None, check=False)
+    fwd = lambda a, out: capi.call("fms_ssm_forward", a, out, None, None, None, 0, None, check=False)
     assert fwd(None, p) == capi.FMS_ERR_NULL_POINTER
     assert fwd(a, None) == capi.FMS_ERR_NULL_POINTER
     assert fwd(ssm_args(p, delta=p + 2), p) == capi.FMS_ERR_MISALIGNED
