@@ -74,14 +74,14 @@ size_t ssm_carry_smem(const fms_ssm_args *a, int cw) {
 // over more work (and, backward, shrink the partial sums of their gradients); fewer, and more pieces of
 // time, give more CTAs, but pieces cost a first pass over the data, a fold and two launches.  The cut with
 // the least expected time is taken.  Measured on B200 (16-bit types, N = 16): a CTA's tile takes
-// (channels of a warp + 1.5) x `unit[n - 1]` microseconds with n CTAs on an SM; a cut time takes `again`
+// (channels of a warp + `own`) x `unit[n - 1]` microseconds with n CTAs on an SM; a cut time takes `again`
 // as long, plus `fixed` for its launches.
 struct CutCosts {
     int warps, per_sm;
-    double unit[3], again, fixed;
+    double own, unit[2], again, fixed;
 };
-constexpr CutCosts kFwdCosts{fms::kSsmFwdWarps, 3, {0.68, 0.80, 1.08}, 1.7, 12};
-constexpr CutCosts kBwdCosts{fms::kSsmBwdWarps, 1, {2.14, 2.14, 2.14}, 1.32, 14};
+constexpr CutCosts kFwdCosts{fms::kSsmFwdWarps, 2, 1.9, {0.55, 0.66}, 1.75, 12};
+constexpr CutCosts kBwdCosts{fms::kSsmBwdWarps, 1, 1.5, {1.85, 1.85}, 1.4, 14};
 
 struct SsmCut {
     int cw, segs, seg_tiles;
@@ -104,7 +104,7 @@ SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const f
             const int64_t len = (tiles + segs - 1) / segs;
             segs = (tiles + len - 1) / len;
             const int64_t full = ctas * segs / (most * sms), rest = (ctas * segs - full * most * sms + sms - 1) / sms;
-            double t = (full * k.unit[most - 1] + (rest ? k.unit[rest - 1] : 0)) * len * (cw + 1.5);
+            double t = (full * k.unit[most - 1] + (rest ? k.unit[rest - 1] : 0)) * len * (cw + k.own);
             if (segs > 1) t = t * k.again + k.fixed;
             if (least == 0 || t < least) best = SsmCut{cw, static_cast<int>(segs), static_cast<int>(len)}, least = t;
         }

@@ -333,23 +333,41 @@ __device__ __forceinline__ f2 lane_move(f2 v, int k) {
     return UP ? pk(__shfl_up_sync(kFullMask, lo(v), k, 8), __shfl_up_sync(kFullMask, hi(v), k, 8))
               : pk(__shfl_down_sync(kFullMask, lo(v), k, 8), __shfl_down_sync(kFullMask, hi(v), k, 8));
 }
-template <bool UP>
-__device__ __forceinline__ f2 lane_scan2(f2 P, f2 &S, f2 carry, int s) {
+// M scans side by side: P, S as in lane_scan; carry[k][j] goes in, and the state after all lanes' positions
+// comes out in the last lane's; in[k] is the state that enters the lane.
+template <int M>
+struct Count {
+    static constexpr int value = M;
+};
+template <bool UP, int M>
+__device__ __forceinline__ void lane_scan2(f2 (&P)[M], f2 (&S)[M], f2 (&carry)[M][2], int j, f2 (&in)[M], int s) {
     const int r = UP ? s : 7 - s;
-    if (r == 0) S = fma2(P, carry, S);
 #pragma unroll
-    for (int k = 1; k < 8; k *= 2) {
-        const f2 Sp = lane_move<UP>(S, k);
-        f2 Pp = 0;
-        if (k < 4) Pp = lane_move<UP>(P, k);
-        if (r >= k) {
-            S = fma2(P, Sp, S);
-            if (k < 4) P = mul2(P, Pp);
+    for (int k = 0; k < M; ++k)
+        if (r == 0) S[k] = fma2(P[k], carry[k][j], S[k]);
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) {
+        f2 Sp[M], Pp[M];
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+            Sp[k] = lane_move<UP>(S[k], d);
+            if (d < 4) Pp[k] = lane_move<UP>(P[k], d);
         }
+#pragma unroll
+        for (int k = 0; k < M; ++k)
+            if (r >= d) {
+                S[k] = fma2(P[k], Sp[k], S[k]);
+                if (d < 4) P[k] = mul2(P[k], Pp[k]);
+            }
     }
-    const f2 in = lane_move<UP>(S, 1);
-    return r == 0 ? carry : in;
+#pragma unroll
+    for (int k = 0; k < M; ++k) {
+        const f2 v = lane_move<UP>(S[k], 1);
+        in[k] = r == 0 ? carry[k][j] : v;
+        carry[k][j] = S[k];
+    }
 }
+
 // Which channels a warp has: [c0, c0 + nc) of group g of sequence b; nc may be <= 0.
 struct SsmPlace {
     int64_t b, d0;  // sequence; first channel counted over all groups
@@ -458,7 +476,7 @@ struct SsmWalk {
 };
 
 template <typename S, bool ALIGNED>
-__global__ void __launch_bounds__(kSsmFwdWarps * 32, 3)
+__global__ void __launch_bounds__(kSsmFwdWarps * 32, 2)
 ssm_forward_kernel(const SsmProblem<S> p, const float *__restrict__ carries, S *__restrict__ out,
                    float *__restrict__ h_last, float *__restrict__ checkpoints) {
     extern __shared__ __align__(16) unsigned char ssm_smem[];
@@ -561,44 +579,64 @@ ssm_forward_kernel(const SsmProblem<S> p, const float *__restrict__ carries, S *
                     zip8(e, o, C[j]);
                 }
             }
-            for (int c = 0; c < w.nc; ++c) {
-                f2 dt[8], u[8], y[8];
-                tile_get_twice(dt_ + c * kSsmTile, s, dt);
-                tile_get_twice(u_ + c * kSsmTile, s, u);
-                const f2 span = add2(add2(add2(dt[0], dt[1]), add2(dt[2], dt[3])), add2(add2(dt[4], dt[5]), add2(dt[6], dt[7])));
-                const float4 A4 = *reinterpret_cast<const float4 *>(A_ + c * p.NP + n0);
-                const float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
+            // M channels side by side: their chains of multiply-adds and shuffles overlap
+            auto channels = [&](int c, auto m) {
+                constexpr int M = decltype(m)::value;
+                f2 dt[M][8], u[M][8], Av[M][2], hv[M][2], span[M];
+                float y[M][8];
+#pragma unroll
+                for (int k = 0; k < M; ++k) {
+                    tile_get_twice(dt_ + (c + k) * kSsmTile, s, dt[k]);
+                    tile_get_twice(u_ + (c + k) * kSsmTile, s, u[k]);
+                    const float4 A4 = *reinterpret_cast<const float4 *>(A_ + (c + k) * p.NP + n0);
+                    const float4 h4 = *reinterpret_cast<const float4 *>(h_ + (c + k) * p.NP + n0);
+                    Av[k][0] = pk(A4.x, A4.y), Av[k][1] = pk(A4.z, A4.w);
+                    hv[k][0] = pk(h4.x, h4.y), hv[k][1] = pk(h4.z, h4.w);
+                    span[k] = add2(add2(add2(dt[k][0], dt[k][1]), add2(dt[k][2], dt[k][3])),
+                                   add2(add2(dt[k][4], dt[k][5]), add2(dt[k][6], dt[k][7])));
+                }
                 __syncwarp();  // the carries are read before the last time lane replaces them
-                const f2 Av[2] = {pk(A4.x, A4.y), pk(A4.z, A4.w)};
-                f2 hv[2] = {pk(h4.x, h4.y), pk(h4.z, h4.w)};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    f2 a[8], b[8];
+                    f2 a[M][8], b[M][8], P[M], S0[M], h[M];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const f2 e = mul2(dt[i], Av[j]);
-                        a[i] = pk(ex2(lo(e)), ex2(hi(e)));
-                        b[i] = mul2(u[i], B[j][i]);
+                    for (int k = 0; k < M; ++k) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const f2 e = mul2(dt[k][i], Av[k][j]);
+                            a[k][i] = pk(ex2(lo(e)), ex2(hi(e)));
+                            b[k][i] = mul2(u[k][i], B[j][i]);
+                        }
+                        const f2 e = mul2(span[k], Av[k][j]);
+                        P[k] = pk(ex2(lo(e)), ex2(hi(e)));
+                        S0[k] = b[k][0];
                     }
-                    const f2 e = mul2(span, Av[j]), P = pk(ex2(lo(e)), ex2(hi(e)));
-                    f2 S0 = b[0];
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) S0 = fma2(a[i], S0, b[i]);
-                    f2 h = lane_scan2<true>(P, S0, hv[j], s);
-                    hv[j] = S0;
+                    for (int i = 1; i < 8; ++i)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        h = fma2(a[i], h, b[i]);
-                        y[i] = j ? fma2(C[j][i], h, y[i]) : mul2(C[j][i], h);
-                    }
+                        for (int k = 0; k < M; ++k) S0[k] = fma2(a[k][i], S0[k], b[k][i]);
+                    lane_scan2<true, M>(P, S0, hv, j, h, s);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int k = 0; k < M; ++k) {
+                            h[k] = fma2(a[k][i], h[k], b[k][i]);
+                            y[k][i] = j ? fmaf(lo(C[j][i]), lo(h[k]), y[k][i]) : lo(C[j][i]) * lo(h[k]);
+                            y[k][i] = fmaf(hi(C[j][i]), hi(h[k]), y[k][i]);
+                        }
                 }
-                if (s == 7)
-                    *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(lo(hv[0]), hi(hv[0]), lo(hv[1]), hi(hv[1]));
-                f2 sum[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = pk(lo(y[2 * k]) + hi(y[2 * k]), lo(y[2 * k + 1]) + hi(y[2 * k + 1]));
-                tile_sum(y_ + c * kSsmTile, s, q, sum, nb == 0);
-            }
+                for (int k = 0; k < M; ++k) {
+                    if (s == 7)
+                        *reinterpret_cast<float4 *>(h_ + (c + k) * p.NP + n0) =
+                            make_float4(lo(hv[k][0]), hi(hv[k][0]), lo(hv[k][1]), hi(hv[k][1]));
+                    const f2 sum[4] = {pk(y[k][0], y[k][1]), pk(y[k][2], y[k][3]), pk(y[k][4], y[k][5]), pk(y[k][6], y[k][7])};
+                    tile_sum(y_ + (c + k) * kSsmTile, s, q, sum, nb == 0);
+                }
+            };
+            int c = 0;
+            for (; c + 1 < w.nc; c += 2) channels(c, Count<2>{});
+            if (c < w.nc) channels(c, Count<1>{});
         }
         __syncwarp();
         for (int c = lane >> 4; c < w.nc; c += 2) {
@@ -1086,23 +1124,22 @@ ssm_carry_kernel(const SsmProblem<S> p, const S *__restrict__ grad_out, float *_
             const float4 h4 = *reinterpret_cast<const float4 *>(h_ + c * p.NP + n0);
             __syncwarp();
             const f2 Av[2] = {pk(A4.x, A4.y), pk(A4.z, A4.w)};
-            f2 hv[2] = {pk(h4.x, h4.y), pk(h4.z, h4.w)};
+            f2 hv[1][2] = {{pk(h4.x, h4.y), pk(h4.z, h4.w)}};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const f2 all = mul2(span, Av[j]), P = pk(ex2(lo(all)), ex2(hi(all)));
-                f2 S0 = 0;
+                const f2 all = mul2(span, Av[j]);
+                f2 P[1] = {pk(ex2(lo(all)), ex2(hi(all)))}, S0[1] = {0}, in[1];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int i8 = REVERSE ? 7 - k : k;
                     const f2 e = mul2(dt[i8], Av[j]), a = pk(ex2(lo(e)), ex2(hi(e))), b = mul2(u[i8], V[j][i8]);
                     // h = a h + u B;  reverse c = a (C dy + c)
-                    S0 = REVERSE ? mul2(a, k ? add2(S0, b) : b) : (k ? fma2(a, S0, b) : b);
+                    S0[0] = REVERSE ? mul2(a, k ? add2(S0[0], b) : b) : (k ? fma2(a, S0[0], b) : b);
                 }
-                lane_scan2<!REVERSE>(P, S0, hv[j], s);
-                hv[j] = S0;
+                lane_scan2<!REVERSE, 1>(P, S0, hv, j, in, s);
             }
             if (s == (REVERSE ? 0 : 7))
-                *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(lo(hv[0]), hi(hv[0]), lo(hv[1]), hi(hv[1]));
+                *reinterpret_cast<float4 *>(h_ + c * p.NP + n0) = make_float4(lo(hv[0][0]), hi(hv[0][0]), lo(hv[0][1]), hi(hv[0][1]));
         }
     }
     __syncwarp();
