@@ -308,24 +308,37 @@ __device__ __forceinline__ void tile_sum(float *base, int s, int q, const f2 (&v
     *at = o;
 }
 
-// Inclusive scan of (P, S) over the 8 time lanes, towards higher or lower lanes; the first lane's S is
-// already the true state.  Returns the state that enters the lane; `S` becomes the one that leaves it.
-template <bool UP>
-__device__ __forceinline__ float lane_scan(float P, float &S, float carry, int s) {
+// Inclusive scans of M pairs (P, S) over the 8 time lanes, towards higher or lower lanes, side by side;
+// `carry` enters the first lane.  in: the state that enters the lane; S becomes the one that leaves it.
+template <bool UP, int M>
+__device__ __forceinline__ void lane_scan(const float (&P0)[M], float (&S)[M], const float (&carry)[M], float (&in)[M], int s) {
     const int r = UP ? s : 7 - s;
-    if (r == 0) S = fmaf(P, carry, S);
+    float P[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        P[m] = P0[m];
+        if (r == 0) S[m] = fmaf(P[m], carry[m], S[m]);
+    }
 #pragma unroll
     for (int k = 1; k < 8; k *= 2) {
-        const float Sp = UP ? __shfl_up_sync(kFullMask, S, k, 8) : __shfl_down_sync(kFullMask, S, k, 8);
-        float Pp = 0.f;
-        if (k < 4) Pp = UP ? __shfl_up_sync(kFullMask, P, k, 8) : __shfl_down_sync(kFullMask, P, k, 8);
-        if (r >= k) {
-            S = fmaf(P, Sp, S);
-            P *= Pp;
+        float Sp[M], Pp[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            Sp[m] = UP ? __shfl_up_sync(kFullMask, S[m], k, 8) : __shfl_down_sync(kFullMask, S[m], k, 8);
+            if (k < 4) Pp[m] = UP ? __shfl_up_sync(kFullMask, P[m], k, 8) : __shfl_down_sync(kFullMask, P[m], k, 8);
         }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+            if (r >= k) {
+                S[m] = fmaf(P[m], Sp[m], S[m]);
+                if (k < 4) P[m] *= Pp[m];
+            }
     }
-    const float in = UP ? __shfl_up_sync(kFullMask, S, 1, 8) : __shfl_down_sync(kFullMask, S, 1, 8);
-    return r == 0 ? carry : in;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        const float v = UP ? __shfl_up_sync(kFullMask, S[m], 1, 8) : __shfl_down_sync(kFullMask, S[m], 1, 8);
+        in[m] = r == 0 ? carry[m] : v;
+    }
 }
 // The same for two states at once, packed.
 template <bool UP>
@@ -690,10 +703,10 @@ template <typename S, bool ALIGNED, bool GATED>
 __global__ void __launch_bounds__(kSsmBwdWarps * 32, 1)
 ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
     extern __shared__ __align__(16) unsigned char ssm_smem[];
-    constexpr int W = kSsmBwdWarps, RB = row_bytes<S>();
+    constexpr int W = kSsmBwdWarps, RB = row_bytes<S>(), NL = 2;  // states of a lane, side by side
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = lane & 7, q = lane >> 3;
     const SsmPlace w = ssm_place(p, W);
-    float *red = reinterpret_cast<float *>(ssm_smem + ssm_bc_bytes<S>());  // [warp][64][lane]
+    float *red = reinterpret_cast<float *>(ssm_smem + ssm_bc_bytes<S>());  // [2][warp][32][lane]
     unsigned char *raw = reinterpret_cast<unsigned char *>(red + W * 64 * 32) + warp * ssm_bwd_warp_bytes<S>(p.cw, p.NP);
     const int ct = p.cw * kSsmTile, cn = p.cw * p.NP;
     float *ck_ = reinterpret_cast<float *>(raw + kSsmStages * 4 * p.cw * RB), *dt_ = ck_ + kSsmStages * cn;
@@ -830,124 +843,129 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                 }
                 __syncwarp();
             }
-            const int n0 = nb * kSsmNB + q * kSsmNL;
-            f2 B[kSsmNL][4], C[kSsmNL][4], dB[kSsmNL][4], dC[kSsmNL][4];
-            {
+            for (int sub = 0; sub < kSsmNB && nb * kSsmNB + sub < p.N; sub += 4 * NL) {  // 8 states at a time
+                const int n0 = nb * kSsmNB + sub + q * NL;
+                const bool fresh = nb == 0 && sub == 0;
+                f2 B[NL][4], C[NL][4], dB[NL][4], dC[NL][4];
 #pragma unroll
-                for (int j = 0; j < kSsmNL; ++j) {
-                    const int r = q * kSsmNL + j;
+                for (int j = 0; j < NL; ++j) {
+                    const int r = sub + q * NL + j;
                     row_eight<S, ALIGNED>(bc + r * RB, row_shift<S, ALIGNED>(Brow + (n0 + j) * p.Bs[2]), s, B[j]);
                     row_eight<S, ALIGNED>(bc + (kSsmNB + r) * RB, row_shift<S, ALIGNED>(Crow + (n0 + j) * p.Cs[2]), s, C[j]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) dB[j][k] = dC[j][k] = 0;
                 }
-            }
-            for (int c = 0; c < w.nc; ++c) {
-                f2 dt[4], u[4], dy[4], gB[4], Q[4], y[4];
-                float dA[kSsmNL];
-                tile_get(dt_ + c * kSsmTile, s, dt);
-                tile_get(u_ + c * kSsmTile, s, u);
-                tile_get(dy_ + c * kSsmTile, s, dy);
-                const f2 both = add2(add2(dt[0], dt[1]), add2(dt[2], dt[3]));
-                const float sum = lo(both) + hi(both);
-                const int at = c * p.NP + n0;
-                const float4 A4 = *reinterpret_cast<const float4 *>(A_ + at), h4 = *reinterpret_cast<const float4 *>(h_ + at);
-                const float4 c4 = *reinterpret_cast<const float4 *>(c_ + at);
-                __syncwarp();  // the carries are read before the first time lane replaces them
-                const float Av[4] = {A4.x, A4.y, A4.z, A4.w}, hv[4] = {h4.x, h4.y, h4.z, h4.w};
-                float cv[4] = {c4.x, c4.y, c4.z, c4.w};
+                for (int c = 0; c < w.nc; ++c) {
+                    f2 dt[4], u[4], dy[4], gB[4], Q[4], y[4];
+                    float dA[NL];
+                    tile_get(dt_ + c * kSsmTile, s, dt);
+                    tile_get(u_ + c * kSsmTile, s, u);
+                    tile_get(dy_ + c * kSsmTile, s, dy);
+                    const f2 both = add2(add2(dt[0], dt[1]), add2(dt[2], dt[3]));
+                    const float sum = lo(both) + hi(both);
+                    const int at = c * p.NP + n0;
+                    const float2 A2 = *reinterpret_cast<const float2 *>(A_ + at), h2 = *reinterpret_cast<const float2 *>(h_ + at);
+                    const float2 c2 = *reinterpret_cast<const float2 *>(c_ + at);
+                    __syncwarp();  // the carries are read before the first time lane replaces them
+                    const float Av[NL] = {A2.x, A2.y}, hv[NL] = {h2.x, h2.y};
+                    float cv[NL] = {c2.x, c2.y};
+                    f2 a[NL][4], v[NL][4], h[NL][4], e[NL][4];
+                    float P[NL], S0[NL], hin[NL], after[NL];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) gB[k] = Q[k] = y[k] = 0;
+                    for (int k = 0; k < 4; ++k) gB[k] = Q[k] = y[k] = 0;
 #pragma unroll
-                for (int j = 0; j < kSsmNL; ++j) {
-                    const f2 Ad = pk(Av[j], Av[j]);
-                    f2 a[4], v[4];
+                    for (int j = 0; j < NL; ++j) {
+                        const f2 Ad = pk(Av[j], Av[j]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const f2 x = mul2(dt[k], Ad);
+                            a[j][k] = pk(ex2(lo(x)), ex2(hi(x)));
+                            v[j][k] = mul2(u[k], B[j][k]);
+                        }
+                        P[j] = ex2(sum * Av[j]);
+                        S0[j] = lo(v[j][0]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            if (k) S0[j] = fmaf(lo(a[j][k]), S0[j], lo(v[j][k]));
+                            S0[j] = fmaf(hi(a[j][k]), S0[j], hi(v[j][k]));
+                        }
+                    lane_scan<true, NL>(P, S0, hv, hin, s);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            const float h1 = fmaf(lo(a[j][k]), k ? hi(h[j][k ? k - 1 : 0]) : hin[j], lo(v[j][k]));
+                            h[j][k] = pk(h1, fmaf(hi(a[j][k]), h1, hi(v[j][k])));
+                            dC[j][k] = fma2(dy[k], h[j][k], dC[j][k]);
+                            if (GATED) y[k] = fma2(C[j][k], h[j][k], y[k]);
+                            e[j][k] = mul2(C[j][k], dy[k]);
+                            v[j][k] = mul2(a[j][k], e[j][k]);
+                        }
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) S0[j] = hi(v[j][3]);
+#pragma unroll
+                    for (int k = 3; k >= 0; --k)
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            if (k < 3) S0[j] = fmaf(hi(a[j][k]), S0[j], hi(v[j][k]));
+                            S0[j] = fmaf(lo(a[j][k]), S0[j], lo(v[j][k]));
+                        }
+                    lane_scan<false, NL>(P, S0, cv, after, s);  // c of the position behind
+                    if (s == 0) *reinterpret_cast<float2 *>(c_ + at) = make_float2(S0[0], S0[1]);
+                    f2 dAj[NL] = {0, 0};
+#pragma unroll
+                    for (int k = 3; k >= 0; --k)
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) {
+                            const float c1 = fmaf(hi(a[j][k]), after[j], hi(v[j][k])), c0 = fmaf(lo(a[j][k]), c1, lo(v[j][k]));
+                            const f2 g = add2(e[j][k], pk(c1, after[j]));
+                            const f2 qq = pk(c0 * (k ? hi(h[j][k ? k - 1 : 0]) : hin[j]), c1 * lo(h[j][k]));
+                            after[j] = c0;
+                            Q[k] = fma2(pk(Av[j], Av[j]), qq, Q[k]);
+                            dAj[j] = fma2(dt[k], qq, dAj[j]);
+                            gB[k] = fma2(g, B[j][k], gB[k]);
+                            dB[j][k] = fma2(g, u[k], dB[j][k]);
+                        }
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) dA[j] = lo(dAj[j]) + hi(dAj[j]);
+                    {  // dA over the 8 time lanes: lane s < 2 keeps state s
+                        float d = ((s & 1) ? dA[1] : dA[0]) + __shfl_xor_sync(kFullMask, (s & 1) ? dA[0] : dA[1], 1);
+                        d += __shfl_xor_sync(kFullMask, d, 2);
+                        d += __shfl_xor_sync(kFullMask, d, 4);
+                        if (s < 2) dA_[at + s] += d;
+                    }
+                    tile_sum(gB_ + c * kSsmTile, s, q, gB, fresh);
+                    tile_sum(q_ + c * kSsmTile, s, q, Q, fresh);
+                    if (GATED) tile_sum(y_ + c * kSsmTile, s, q, y, fresh);
+                }
+                // dB, dC over the warps of the CTA; the two halves of `red` take turns
+                float *half = red + ((sub / (4 * NL)) & 1) * W * 32 * 32, *slot = half + warp * 32 * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < NL; ++j)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const f2 x = mul2(dt[k], Ad);
-                        a[k] = pk(ex2(lo(x)), ex2(hi(x)));
-                        v[k] = mul2(u[k], B[j][k]);
+                        slot[(j * 8 + 2 * k) * 32] = lo(dB[j][k]);
+                        slot[(j * 8 + 2 * k + 1) * 32] = hi(dB[j][k]);
+                        slot[((NL + j) * 8 + 2 * k) * 32] = lo(dC[j][k]);
+                        slot[((NL + j) * 8 + 2 * k + 1) * 32] = hi(dC[j][k]);
                     }
-                    float S0 = lo(v[0]);
+                __syncthreads();
+                {
+                    static_assert(W == 4 * NL, "a warp sums four positions of one state of dB or dC");
+                    const int n = n0 + ((warp >> 1) & (NL - 1)), which = warp / (2 * NL);
+                    float x[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k) S0 = fmaf(lo(a[k]), S0, lo(v[k]));
-                        S0 = fmaf(hi(a[k]), S0, hi(v[k]));
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = 0.f;
+#pragma unroll
+                        for (int k = 0; k < W; ++k) x[i] += half[(k * 32 + warp * 4 + i) * 32 + lane];
                     }
-                    const float P = ex2(sum * Av[j]);
-                    const float hin = lane_scan<true>(P, S0, hv[j], s);
-                    f2 h[4], e[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float h1 = fmaf(lo(a[k]), k ? hi(h[k ? k - 1 : 0]) : hin, lo(v[k]));
-                        h[k] = pk(h1, fmaf(hi(a[k]), h1, hi(v[k])));
-                        dC[j][k] = fma2(dy[k], h[k], dC[j][k]);
-                        if (GATED) y[k] = fma2(C[j][k], h[k], y[k]);
-                        e[k] = mul2(C[j][k], dy[k]);
-                        v[k] = mul2(a[k], e[k]);
-                    }
-                    float R0 = hi(v[3]);
-#pragma unroll
-                    for (int k = 3; k >= 0; --k) {
-                        if (k < 3) R0 = fmaf(hi(a[k]), R0, hi(v[k]));
-                        R0 = fmaf(lo(a[k]), R0, lo(v[k]));
-                    }
-                    float after = lane_scan<false>(P, R0, cv[j], s);  // c of the position behind
-                    cv[j] = R0;
-                    f2 dAj = 0;
-#pragma unroll
-                    for (int k = 3; k >= 0; --k) {
-                        const float c1 = fmaf(hi(a[k]), after, hi(v[k])), c0 = fmaf(lo(a[k]), c1, lo(v[k]));
-                        const f2 g = add2(e[k], pk(c1, after));
-                        const f2 qq = pk(c0 * (k ? hi(h[k ? k - 1 : 0]) : hin), c1 * lo(h[k]));
-                        after = c0;
-                        Q[k] = fma2(Ad, qq, Q[k]);
-                        dAj = fma2(dt[k], qq, dAj);
-                        gB[k] = fma2(g, B[j][k], gB[k]);
-                        dB[j][k] = fma2(g, u[k], dB[j][k]);
-                    }
-                    dA[j] = lo(dAj) + hi(dAj);
-                }
-                if (s == 0) *reinterpret_cast<float4 *>(c_ + at) = make_float4(cv[0], cv[1], cv[2], cv[3]);
-                {  // dA over the 8 time lanes: lane s < 4 keeps state 2 * (s & 1) + (s >> 1)
-                    const bool up = s & 1, up2 = s & 2;
-                    const float r0 = (up ? dA[2] : dA[0]) + __shfl_xor_sync(kFullMask, up ? dA[0] : dA[2], 1);
-                    const float r1 = (up ? dA[3] : dA[1]) + __shfl_xor_sync(kFullMask, up ? dA[1] : dA[3], 1);
-                    float d = (up2 ? r1 : r0) + __shfl_xor_sync(kFullMask, up2 ? r0 : r1, 2);
-                    d += __shfl_xor_sync(kFullMask, d, 4);
-                    if (s < 4) dA_[at + 2 * (s & 1) + (s >> 1)] += d;
-                }
-                tile_sum(gB_ + c * kSsmTile, s, q, gB, nb == 0);
-                tile_sum(q_ + c * kSsmTile, s, q, Q, nb == 0);
-                if (GATED) tile_sum(y_ + c * kSsmTile, s, q, y, nb == 0);
-            }
-            // dB, dC over the warps of the CTA
-            float *slot = red + warp * 64 * 32 + lane;
-#pragma unroll
-            for (int j = 0; j < kSsmNL; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    slot[(j * 8 + 2 * k) * 32] = lo(dB[j][k]);
-                    slot[(j * 8 + 2 * k + 1) * 32] = hi(dB[j][k]);
-                    slot[((4 + j) * 8 + 2 * k) * 32] = lo(dC[j][k]);
-                    slot[((4 + j) * 8 + 2 * k + 1) * 32] = hi(dC[j][k]);
-                }
-            __syncthreads();
-            {
-                static_assert(W == 2 * kSsmNL, "a warp sums the values of one state of dB or dC");
-                const int n = n0 + (warp & 3);
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[i] = 0.f;
-#pragma unroll
-                    for (int k = 0; k < W; ++k) v[i] += red[(k * 64 + warp * 8 + i) * 32 + lane];
-                }
-                if (n < p.N) {
-                    float4 *to = reinterpret_cast<float4 *>(bc_out + (static_cast<int64_t>(warp >> 2) * p.N + n) * Tpad +
-                                                            tile * kSsmTile + s * kSsmE);
-                    to[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    to[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    if (n < p.N)
+                        *reinterpret_cast<float4 *>(bc_out + (static_cast<int64_t>(which) * p.N + n) * Tpad + tile * kSsmTile +
+                                                    s * kSsmE + 4 * (warp & 1)) = make_float4(x[0], x[1], x[2], x[3]);
                 }
             }
         }
