@@ -3,7 +3,6 @@
 #include "fm_scan_b200.h"
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "capi_common.cuh"
 #include "ssm_kernels.cuh"
@@ -47,7 +46,6 @@ inline int padded_states(const fms_ssm_args *a) {
     return static_cast<int>((a->states + fms::kSsmNB - 1) / fms::kSsmNB * fms::kSsmNB);
 }
 
-int env_int(const char *name, int dflt) { const char *s = std::getenv(name); return s ? std::atoi(s) : dflt; }
 // shared memory of a CTA: as the kernels lay it out
 template <typename F>
 size_t by_width(const fms_ssm_args *a, F f) { return a->dtype == FMS_F32 ? f(float{}) : f(__half{}); }
@@ -86,7 +84,7 @@ constexpr CutCosts kBwdCosts{fms::kSsmBwdWarps, 1, 1.5, {1.85, 1.85}, 1.4, 14};
 struct SsmCut {
     int cw, segs, seg_tiles;
 };
-SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const fms_ssm_args *, int), int force_cw, int force_segs) {
+SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const fms_ssm_args *, int)) {
     const int64_t per = a->channels / a->groups, sms = 148;
     const int tiles = static_cast<int>((a->T + fms::kSsmTile - 1) / fms::kSsmTile);
     SsmCut best{1, 1, tiles};
@@ -94,13 +92,11 @@ SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const f
     for (int cw = 1; cw <= 8; ++cw) {
         const size_t bytes = smem(a, cw);
         if (bytes > kMaxSmem) break;
-        if (force_cw && cw != force_cw) continue;
         const int64_t ctas = a->batch * a->groups * ((per + cw * k.warps - 1) / (cw * k.warps));
         const int64_t most = std::min<int64_t>(k.per_sm, static_cast<int64_t>((kMaxSmem + 1024) / (bytes + 1024)));
         for (int waves = 0; waves <= 4; ++waves) {  // 0: time is not cut; else as many pieces as fill the waves
             int64_t segs = waves ? std::min<int64_t>(tiles, waves * most * sms / ctas) : 1;
-            if (force_segs) segs = std::min(tiles, force_segs);
-            if (segs < 1 || (waves && segs < 2 && !force_segs)) continue;
+            if (segs < (waves ? 2 : 1)) continue;
             const int64_t len = (tiles + segs - 1) / segs;
             segs = (tiles + len - 1) / len;
             const int64_t full = ctas * segs / (most * sms), rest = (ctas * segs - full * most * sms + sms - 1) / sms;
@@ -111,8 +107,8 @@ SsmCut best_cut(const fms_ssm_args *a, const CutCosts &k, size_t (*smem)(const f
     }
     return best;
 }
-SsmCut ssm_fwd_cut(const fms_ssm_args *a) { return best_cut(a, kFwdCosts, ssm_fwd_smem, env_int("X_FCW", 0), env_int("X_FSEG", 0)); }
-SsmCut ssm_bwd_cut(const fms_ssm_args *a) { return best_cut(a, kBwdCosts, ssm_bwd_smem, env_int("X_BCW", 0), env_int("X_BSEG", 0)); }
+SsmCut ssm_fwd_cut(const fms_ssm_args *a) { return best_cut(a, kFwdCosts, ssm_fwd_smem); }
+SsmCut ssm_bwd_cut(const fms_ssm_args *a) { return best_cut(a, kBwdCosts, ssm_bwd_smem); }
 
 template <typename S>
 fms::SsmProblem<S> ssm_problem(const fms_ssm_args *a, const SsmCut &cut, int warps) {
@@ -233,27 +229,23 @@ int launch_ssm_backward(const fms_ssm_args *a, fms::SsmGrads<S> o, S *dB, S *dC,
     return check_launch();
 }
 
-template <typename S, bool VEC, int U>
-int launch_ssm_step_u(const fms::SsmProblem<S> &p, float *state, int64_t pool, const int64_t *slots, void *out, int log_L,
-                      cudaStream_t st) {
+template <typename S, bool VEC>
+int launch_ssm_step_v(const fms::SsmProblem<S> &p, float *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
+    int log_L = 0;  // lanes of a channel: 8 states each
+    while (log_L < 5 && (8 << log_L) < p.N) ++log_L;
     const int per = 128 >> log_L;
-    const dim3 grid(static_cast<unsigned>((p.per_group + per * U - 1) / (per * U)), static_cast<unsigned>(p.groups),
+    const dim3 grid(static_cast<unsigned>((p.per_group + per - 1) / per), static_cast<unsigned>(p.groups),
                     static_cast<unsigned>(std::min<int64_t>(p.batch, 65535)));
     const bool bc_vec = p.N % 8 == 0 && rows16(p.B, p.Bs, 2, sizeof(S)) && rows16(p.C, p.Cs, 2, sizeof(S));
-    fms::ssm_step_kernel<S, VEC, U><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), log_L, bc_vec);
+    fms::ssm_step_kernel<S, VEC><<<grid, 128, 0, st>>>(p, state, pool, slots, static_cast<S *>(out), log_L, bc_vec);
     return check_launch();
 }
 template <typename S>
 int launch_ssm_step(const fms_ssm_args *a, float *state, int64_t pool, const int64_t *slots, void *out, cudaStream_t st) {
     const auto p = ssm_problem<S>(a, SsmCut{1, 1, 1}, 1);
     if (p.groups > 65535) return FMS_ERR_TOO_LARGE;
-    int log_L = 0;
-    while (log_L < 5 && (8 << log_L) < p.N) ++log_L;
-    const bool vec = p.N % 8 == 0 && aligned_to(state, 16) && aligned_to(p.A, 16);
-    const bool many = (p.batch * p.channels << log_L) >= env_int("X_MANY", 148 * 1024);
-    if (vec) return many ? launch_ssm_step_u<S, true, 2>(p, state, pool, slots, out, log_L, st)
-                         : launch_ssm_step_u<S, true, 1>(p, state, pool, slots, out, log_L, st);
-    return launch_ssm_step_u<S, false, 1>(p, state, pool, slots, out, log_L, st);
+    return p.N % 8 == 0 && aligned_to(state, 16) && aligned_to(p.A, 16) ? launch_ssm_step_v<S, true>(p, state, pool, slots, out, st)
+                                                                       : launch_ssm_step_v<S, false>(p, state, pool, slots, out, st);
 }
 
 }  // namespace

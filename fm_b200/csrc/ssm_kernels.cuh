@@ -1271,81 +1271,70 @@ __device__ __forceinline__ void load_eight(const S *__restrict__ p, bool vec, in
     }
 }
 
-// A block has 128 U / L channels of one row and group.  What a channel needs once (time step, gate) is
+// A block has 128 / L channels of one row and group.  What a channel needs once (time step, gate) is
 // prepared by one thread per channel in shared memory while the states, asked for before, are on their
-// way; then L lanes share a channel, 8 states a lane (B and C in registers), U channels a thread.  Bound
-// by the states' bytes (8 per state) for many rows, by the latency of one pass for a few: U = 1 there.
-// VEC: states and A come in vectors.
-template <typename S, bool VEC, int U>
+// way; then L lanes share a channel, 8 states a lane.  Bound by the states' bytes (8 per state) for many
+// rows, by the latency of one pass for a few.  Two channels a thread, or a block that walks several rows with
+// the next one's states on their way, were no faster (256 rows x 2048 channels x 16 states: 24 us of 11 us
+// for the bytes alone).  VEC: states and A come in vectors.
+template <typename S, bool VEC>
 __global__ void __launch_bounds__(128)
 ssm_step_kernel(const SsmProblem<S> p, float *__restrict__ state, int64_t pool, const int64_t *__restrict__ slots,
                 S *__restrict__ out, int log_L, bool bc_vec) {
-    __shared__ float4 once[128 * U];  // dt log2(e), dt x, D x, gate
-    __shared__ float y_[128 * U];
-    const int L = 1 << log_L, per = 128 >> log_L, l = threadIdx.x & (L - 1), c0 = threadIdx.x >> log_L;
-    const int first = blockIdx.x * per * U, nc = min(per * U, p.per_group - first), g = blockIdx.y;
+    __shared__ float4 once[128];  // dt log2(e), dt x, D x, gate
+    __shared__ float y_[128];
+    const int L = 1 << log_L, per = 128 >> log_L, l = threadIdx.x & (L - 1), c = threadIdx.x >> log_L;
+    const int first = blockIdx.x * per, nc = min(per, p.per_group - first), g = blockIdx.y;
     const int64_t d0 = static_cast<int64_t>(g) * p.per_group + first;
     for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
         const int64_t slot = step_slot(slots, b, pool);
         const S *Bp = p.B + b * p.Bs[0] + g * p.Bs[1], *Cp = p.C + b * p.Cs[0] + g * p.Cs[1];
-        float *hp = state + (slot * p.channels + d0 + c0) * p.N;
-        const float *Ap = p.A + (d0 + c0) * p.N;
-        float y[U], h[U][8], A[U][8], B[8], C[8];
+        float *hp = state + (slot * p.channels + d0 + c) * p.N;
+        const float *Ap = p.A + (d0 + c) * p.N;
+        float h[8], A[8], B[8], C[8], y = 0.f;
         auto fetch = [&](int n) {
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (c0 + k * per < nc) {
-                    load_eight(hp + k * per * p.N + n, VEC, p.N - n, h[k]);
-                    load_eight(Ap + k * per * p.N + n, VEC, p.N - n, A[k]);
-                }
+            load_eight(hp + n, VEC, p.N - n, h);
+            load_eight(Ap + n, VEC, p.N - n, A);
             load_eight(Bp + n, bc_vec, p.N - n, B);
             load_eight(Cp + n, bc_vec, p.N - n, C);
         };
         if (slot >= 0) {
-            if (8 * l < p.N) fetch(8 * l);
-            for (int c = threadIdx.x; c < nc; c += 128) {
-                const int64_t d = d0 + c;
+            if (c < nc && 8 * l < p.N) fetch(8 * l);
+            if (static_cast<int>(threadIdx.x) < nc) {
+                const int64_t d = d0 + threadIdx.x;
                 const float x = Store<S>::to_float(p.x[b * p.xs[0] + d]), z = p.z ? Store<S>::to_float(p.z[b * p.zs[0] + d]) : 0.f;
                 float dt = Store<S>::to_float(p.delta[b * p.ds[0] + d]) + (p.bias ? p.bias[d] : 0.f);
                 if (p.softplus) dt = softplus_f(dt);
-                once[c] = make_float4(dt * kLog2e, dt * x, p.D ? p.D[d] * x : 0.f, p.z ? z * sigmoid_f(z) : 1.f);
+                once[threadIdx.x] = make_float4(dt * kLog2e, dt * x, p.D ? p.D[d] * x : 0.f, p.z ? z * sigmoid_f(z) : 1.f);
             }
         }
         const bool use = !slot_taken(slots, b, slot) && slot >= 0;  // the block's barrier too
         if (use) {
+            if (c < nc) {
+                const float2 v = *reinterpret_cast<const float2 *>(&once[c]);
+                for (int n = 8 * l; n < p.N; n += 8 * L) {
+                    if (n != 8 * l) fetch(n);
 #pragma unroll
-            for (int k = 0; k < U; ++k) y[k] = 0.f;
-            for (int n = 8 * l; n < p.N; n += 8 * L) {
-                if (n != 8 * l) fetch(n);
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (c0 + k * per < nc) {
-                        const float2 v = *reinterpret_cast<const float2 *>(&once[c0 + k * per]);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            h[k][i] = fmaf(ex2(v.x * A[k][i]), h[k][i], v.y * B[i]);
-                            y[k] = fmaf(C[i], h[k][i], y[k]);
-                        }
-                        float *to = hp + k * per * p.N + n;
-                        if constexpr (VEC) {
-                            reinterpret_cast<float4 *>(to)[0] = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
-                            reinterpret_cast<float4 *>(to)[1] = make_float4(h[k][4], h[k][5], h[k][6], h[k][7]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (n + i < p.N) to[i] = h[k][i];
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        h[i] = fmaf(ex2(v.x * A[i]), h[i], v.y * B[i]);
+                        y = fmaf(C[i], h[i], y);
                     }
-            }
+                    if constexpr (VEC) {
+                        reinterpret_cast<float4 *>(hp + n)[0] = make_float4(h[0], h[1], h[2], h[3]);
+                        reinterpret_cast<float4 *>(hp + n)[1] = make_float4(h[4], h[5], h[6], h[7]);
+                    } else {
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                for (int i = 1; i < L; i *= 2) y[k] += __shfl_xor_sync(kFullMask, y[k], i);
-                if (l == 0) y_[c0 + k * per] = y[k];
+                        for (int i = 0; i < 8; ++i)
+                            if (n + i < p.N) hp[n + i] = h[i];
+                    }
+                }
             }
+            for (int i = 1; i < L; i *= 2) y += __shfl_xor_sync(kFullMask, y, i);
+            if (l == 0) y_[c] = y;
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < nc; c += 128)
-            out[b * p.channels + d0 + c] = from_float<S>(use ? (y_[c] + once[c].z) * once[c].w : 0.f);
+        if (static_cast<int>(threadIdx.x) < nc)
+            out[b * p.channels + d0 + threadIdx.x] = from_float<S>(use ? (y_[threadIdx.x] + once[threadIdx.x].z) * once[threadIdx.x].w : 0.f);
         __syncthreads();
     }
 }

@@ -397,6 +397,20 @@ def test_step_of_a_wide_batch_finds_repeats_beyond_one_block():
     assert torch.equal(state, once) and torch.equal(y[:700], y1) and not y[700:].any()
 
 
+def test_step_reaches_states_behind_32_bit_offsets():
+    D, N, pool = 2048, 16, 65540                     # 2.1e9 floats
+    state = torch.zeros(pool, D, N, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, d, B, C, A = n(2, D), n(2, D), n(2, N), n(2, N), -torch.rand(D, N, generator=g, device="cuda")
+    small = n(2, D, N)
+    slots = torch.tensor([pool - 1, 65536], device="cuda")
+    state[slots] = small
+    y = fm_b200.ssm_step(x, d, state, A, B, C, delta_softplus=True, slots=slots)
+    y1 = fm_b200.ssm_step(x, d, small, A, B, C, delta_softplus=True)
+    assert torch.equal(y, y1) and torch.equal(state[slots], small) and not state[:65536].any()
+
+
 # ------------------------------------------------------------------------------------- filter ----
 
 
