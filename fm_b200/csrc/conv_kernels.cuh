@@ -12,6 +12,10 @@
 // The K - 1 positions in front of a lane's (for dx: the K - 1 values of dpre behind them) come from the
 // neighbouring lane by shuffle, across tiles from the tile walked before, and only at a unit's border from
 // memory.  Rows shorter than a group share a warp.  What happens at a row's ends is kept out of line.
+//
+// Measured at (8,2048,4096) bf16, 4 taps, SiLU: forward 74 us = 3.6 TB/s, backward 135 us = 3.0 TB/s (bytes alone:
+// 42 and 62 us at the measured copy rate); issue slots bound it, some 170 and 330 instructions for a warp's
+// 256 positions.  Rows of odd length, (3,768,16385) fp16: 47 us = 3.2 TB/s.
 #pragma once
 
 #include "ssm_kernels.cuh"
