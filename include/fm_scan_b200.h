@@ -414,7 +414,8 @@ int fms_tsplit_backward(const void *gates, const void *states, const void *grad_
  *
  * Every large tensor has time as its last axis with stride 1; the other strides are given in elements
  * and need not be those of a contiguous tensor (0 included, for inputs).  Tensors the library writes
- * are contiguous.  lengths[b] (nullable, int64 on the device, clamped to [0, T]) ends sequence b
+ * are contiguous and do not overlap its inputs.  Rows that do not start on a 16-byte boundary are read
+ * from the boundary in front of them (up to 15 bytes of the same 16-byte granule, unused).  lengths[b] (nullable, int64 on the device, clamped to [0, T]) ends sequence b
  * early: positions from there on are never read into a result, their outputs and gradients are zero,
  * and the last state is the state at lengths[b].
  */

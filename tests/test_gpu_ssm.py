@@ -483,6 +483,45 @@ def test_filter_takes_strided_and_offset_rows():
     assert torch.equal(fm_b200.short_conv(t, w), fm_b200.short_conv(x.contiguous(), w))
 
 
+def test_filter_of_no_positions_passes_its_state_on():
+    x = torch.zeros(2, 3, 0, device="cuda", requires_grad=True)
+    w = torch.randn(3, 4, device="cuda", requires_grad=True)
+    x0 = torch.randn(2, 3, 3, device="cuda", requires_grad=True)
+    y, last = fm_b200.short_conv(x, w, initial_state=x0, return_state=True)
+    assert y.shape == (2, 3, 0) and torch.equal(last, x0)
+    up = torch.randn(2, 3, 3, device="cuda")
+    dw, d0 = torch.autograd.grad((y, last), (w, x0), (torch.zeros_like(y), up))
+    assert torch.equal(d0, up) and not dw.any()
+
+
+def test_more_sequences_than_a_grid_axis_holds():
+    Bn, K = 65_600, 4
+    g = torch.Generator(device="cuda").manual_seed(8)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, w, up = n(Bn, 1, 5).requires_grad_(True), n(1, K).requires_grad_(True), n(Bn, 1, 5)
+    y = fm_b200.short_conv(x, w)
+    want = torch.nn.functional.conv1d(torch.nn.functional.pad(x.double(), (K - 1, 0)), w.double()[:, None])
+    # each output is a sum of 4 products
+    assert ((y.double() - want).abs() <= 8 * R.U * 64).all()
+    dx, dw = torch.autograd.grad(y, (x, w), up)
+    wx, ww = torch.autograd.grad(want, (x, w), up.double())
+    assert ((dx - wx).abs() <= 8 * R.U * 64).all()
+    assert ((dw - ww).abs() <= (5 * Bn + 8) ** 0.5 * 64 * R.U * 64 * 5).all()
+    state = n(Bn, 1, K - 1)
+    s2 = state.clone()
+    a = fm_b200.short_conv_step(x[..., 0].detach(), state, w.detach())
+    b = fm_b200.short_conv_step(x[65_500:, :, 0].detach(), s2[65_500:].contiguous(), w.detach())
+    assert torch.equal(a[65_500:], b)
+    h = n(Bn, 1, 8)
+    h2 = h[65_500:].clone()
+    A, bc = -torch.ones(1, 8, device="cuda"), n(Bn, 8)
+    a = fm_b200.ssm_step(x[..., 0].detach(), x[..., 1].detach(), h, A, bc, bc, delta_softplus=True)
+    b = fm_b200.ssm_step(x[65_500:, :, 0].detach(), x[65_500:, :, 1].detach(), h2, A, bc[65_500:], bc[65_500:], delta_softplus=True)
+    assert torch.equal(a[65_500:], b) and torch.equal(h[65_500:], h2)
+    z = fm_b200.ssm_scan(x.detach(), x.detach(), A, n(Bn, 8, 5), n(Bn, 8, 5), delta_softplus=True)
+    assert z.isfinite().all()
+
+
 # -------------------------------------------------------------------------------- all together ----
 
 
