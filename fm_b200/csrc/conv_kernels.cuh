@@ -178,29 +178,25 @@ conv_forward_kernel(const ConvProblem<S> p, S *__restrict__ out, S *__restrict__
                 raw[u] = load8(w.x + t, same && t >= 0 && t + 8 <= w.len);
             }
         };
-        fetch(w.first);
 #pragma unroll
         for (int k = 0; k < K; ++k) wt[k] = w.live ? p.weight[w.d * K + k] : 0.f;
         if (p.bias && w.live) bias = p.bias[w.d];
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) prev[j] = w.l == 0 ? conv_at<S, K>(w, w.t0 + w.first * U * span - (K - 1) + j) : 0.f;
         for (int group = w.first; group < w.last; ++group) {
-            Raw8<S> cur[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) cur[u] = raw[u];
-            if (group + 1 < w.last) fetch(group + 1);
+            fetch(group);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int t = w.t0 + (group * U + u) * span;
                 float f[8], halo[K - 1];
                 Eight y;
-                if (!same || t < 0 || t + 8 > w.len) cur[u] = load8_edge(w.x, w.live ? w.x0 : nullptr, t, w.len, K - 1);
-                unpack8(cur[u], f);
+                if (!same || t < 0 || t + 8 > w.len) raw[u] = load8_edge(w.x, w.live ? w.x0 : nullptr, t, w.len, K - 1);
+                unpack8(raw[u], f);
 #pragma unroll
-                for (int j = 0; j < K - 1; ++j) {  // lane 0 goes on from the tile before; `prev` holds its last inputs
-                    const float mine = f[8 - (K - 1) + j], side = __shfl_up_sync(kFullMask, mine, 1, p.lpr);
+                for (int j = 0; j < K - 1; ++j) {  // lane 0 gets the last lane's, for the next tile
+                    const float side = __shfl_sync(kFullMask, f[8 - (K - 1) + j], w.l + p.lpr - 1, p.lpr);
                     halo[j] = w.l == 0 ? prev[j] : side;
-                    prev[j] = __shfl_sync(kFullMask, mine, p.lpr - 1, p.lpr);
+                    prev[j] = side;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y.f[i] = conv_sum<K>(wt, bias, halo, f, i);
@@ -279,6 +275,7 @@ conv_backward_kernel(const ConvProblem<S> p, const S *__restrict__ dout, const S
             const int tg = w.t0 + group * U * span;
             Raw8<S> fr[U], gr[U];
             S front[K - 1];  // lane 0: the inputs in front of the group
+            float turn[K - 1];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int t = tg + u * span;
@@ -306,11 +303,12 @@ conv_backward_kernel(const ConvProblem<S> p, const S *__restrict__ dout, const S
                     unpack8(fr[u], a);
                     unpack8(gr[u], g);
 #pragma unroll
-                    for (int j = 0; j < K - 1; ++j) {  // lane 0 has its inputs in front from the tile before
-                        const float side = __shfl_up_sync(kFullMask, a[8 - (K - 1) + j], 1, p.lpr);
-                        const float before = u ? __shfl_sync(kFullMask, Store<S>::to_float(fr[u ? u - 1 : 0].s[8 - (K - 1) + j]), p.lpr - 1, p.lpr)
-                                               : Store<S>::to_float(front[j]);
-                        f[j] = halo[j] = w.l == 0 ? before : side;
+                    for (int j = 0; j < K - 1; ++j) {  // lane 0 gets the last lane's of the tile in front
+                        if (u == U - 1) turn[j] = __shfl_sync(kFullMask, a[8 - (K - 1) + j], w.l + p.lpr - 1, p.lpr);
+                        const float side = turn[j];
+                        turn[j] = u ? __shfl_sync(kFullMask, Store<S>::to_float(fr[u ? u - 1 : 0].s[8 - (K - 1) + j]), w.l + p.lpr - 1, p.lpr)
+                                    : Store<S>::to_float(front[j]);
+                        f[j] = halo[j] = w.l == 0 ? turn[j] : side;
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -334,9 +332,9 @@ conv_backward_kernel(const ConvProblem<S> p, const S *__restrict__ dout, const S
                 }
 #pragma unroll
                 for (int j = 0; j < K - 1; ++j) {
-                    const float side = __shfl_down_sync(kFullMask, dp[j], 1, p.lpr);
+                    const float side = __shfl_sync(kFullMask, dp[j], w.l + 1, p.lpr);  // the last lane gets lane 0's
                     dp[8 + j] = w.l == p.lpr - 1 ? behind[j] : side;
-                    behind[j] = __shfl_sync(kFullMask, dp[j], 0, p.lpr);
+                    behind[j] = side;
                 }
                 Eight v;
 #pragma unroll
@@ -409,7 +407,7 @@ conv_step_kernel(const ConvProblem<S> p, S *__restrict__ state, int64_t pool, co
         for (int k = 0; k < K; ++k) wt[k] = p.weight[d * K + k];
         if (p.bias) y = p.bias[d];
     }
-    const bool taken = slot_taken(slots, b, slot);
+    const bool taken = __syncthreads_or(slot_seen(slots, b, slot));
     if (use && !taken) {
 #pragma unroll
         for (int k = 0; k < K; ++k) y = fmaf(wt[k], Store<S>::to_float(v[k]), y);

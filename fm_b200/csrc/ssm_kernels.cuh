@@ -1251,17 +1251,17 @@ ssm_finish_kernel(const SsmProblem<S> p, const SsmGrads<S> o, S *__restrict__ dB
 
 // ---------------------------------------------------------------- one token ------------------
 // Row b's place in the pool, or -1 for padding.  A slot that an earlier row names belongs to that row:
-// every thread looks at its share of the earlier rows and the block votes, while the loads of the
-// state that the caller issued before are on their way.
+// every thread looks at its share of the earlier rows, on loads that need not wait for its own slot, and the
+// block votes.
 __device__ __forceinline__ int64_t step_slot(const int64_t *slots, int64_t b, int64_t pool) {
     const int64_t v = slots ? slots[b] : b;
     return v >= 0 && v < pool ? v : -1;
 }
-__device__ __forceinline__ bool slot_taken(const int64_t *slots, int64_t b, int64_t slot) {
+__device__ __forceinline__ bool slot_seen(const int64_t *slots, int64_t b, int64_t slot) {
     bool seen = false;
     if (slots && slot >= 0)
         for (int64_t k = threadIdx.x; k < b; k += blockDim.x) seen |= slots[k] == slot;
-    return __syncthreads_or(seen);
+    return seen;
 }
 
 // Eight consecutive values; `vec`: they are whole and start on a 16-byte boundary.
@@ -1307,6 +1307,7 @@ ssm_step_kernel(const SsmProblem<S> p, float *__restrict__ state, int64_t pool, 
             load_eight(Bp + n, bc_vec, p.N - n, B);
             load_eight(Cp + n, bc_vec, p.N - n, C);
         };
+        const bool seen = slot_seen(slots, b, slot);
         if (slot >= 0) {
             if (c < nc && 8 * l < p.N) fetch(8 * l);
             if (static_cast<int>(threadIdx.x) < nc) {
@@ -1317,7 +1318,7 @@ ssm_step_kernel(const SsmProblem<S> p, float *__restrict__ state, int64_t pool, 
                 once[threadIdx.x] = make_float4(dt * kLog2e, dt * x, p.D ? p.D[d] * x : 0.f, p.z ? z * sigmoid_f(z) : 1.f);
             }
         }
-        const bool use = !slot_taken(slots, b, slot) && slot >= 0;  // the block's barrier too
+        const bool use = !__syncthreads_or(seen) && slot >= 0;
         if (use) {
             if (c < nc) {
                 const float2 v = *reinterpret_cast<const float2 *>(&once[c]);
