@@ -13,9 +13,9 @@
 // neighbouring lane by shuffle, across tiles from the tile walked before, and only at a unit's border from
 // memory.  Rows shorter than a group share a warp.  What happens at a row's ends is kept out of line.
 //
-// Measured at (8,2048,4096) bf16, 4 taps, SiLU: forward 74 us = 3.6 TB/s, backward 135 us = 3.0 TB/s (bytes alone:
-// 42 and 62 us at the measured copy rate); issue slots bound it, some 170 and 330 instructions for a warp's
-// 256 positions.  Rows of odd length, (3,768,16385) fp16: 47 us = 3.2 TB/s.
+// Measured at (8,2048,4096) bf16, 4 taps, SiLU: forward 62 us = 4.3 TB/s, backward 117 us = 3.4 TB/s (bytes alone:
+// 42 and 62 us at the measured copy rate); issue slots bound it, some 170 and 320 instructions for a warp's
+// 256 positions.  Rows of odd length, (3,768,16385) fp16: 40 us = 3.8 TB/s.
 #pragma once
 
 #include "ssm_kernels.cuh"
@@ -160,8 +160,9 @@ __device__ __forceinline__ float conv_sum(const float (&wt)[K], float v, const f
     return v;
 }
 
+// Seven CTAs an SM where the loads of a group are few registers: 68 -> 62 us at (8,2048,4096) bf16.
 template <typename S, int K>
-__global__ void __launch_bounds__(kConvWarps * 32)
+__global__ void __launch_bounds__(kConvWarps * 32, sizeof(S) == 4 ? 4 : K <= 4 ? 7 : 6)
 conv_forward_kernel(const ConvProblem<S> p, S *__restrict__ out, S *__restrict__ x_last) {
     constexpr int U = kConvUnroll;
     const int span = p.lpr * 8;
@@ -234,7 +235,7 @@ __device__ __noinline__ inline Eight keep_inside(Eight v, int t, int len) {
 // part: [unit][row][K + 1], the sums over a unit's positions of dpre * x (K of them) and of dpre.  The groups
 // are walked from the last to the first.
 template <typename S, int K>
-__global__ void __launch_bounds__(kConvWarps * 32)
+__global__ void __launch_bounds__(kConvWarps * 32, sizeof(S) == 4 ? 3 : 4)
 conv_backward_kernel(const ConvProblem<S> p, const S *__restrict__ dout, const S *__restrict__ dlast,
                      S *__restrict__ dx, S *__restrict__ dx0, float *__restrict__ part) {
     constexpr int U = kConvUnroll;
