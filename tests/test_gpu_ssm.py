@@ -177,6 +177,27 @@ def test_scan_ignores_what_stands_behind_a_sequence(junk):
     assert not dB[0].any() and not dC[1, ..., 33:].any()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T, at", [(60, 29), (700, 64), (700, 351), (701, 351)])
+def test_a_bad_position_reaches_no_earlier_output_and_no_later_gradient(T, at, bad):
+    i, grads = scan_case("bf16", 2, 9, T, 16, seed=31)
+    y = call_scan(on_gpu(i))
+    for n in ("x", "delta", "B", "C", "z"):
+        k = {**i, n: i[n].clone()}
+        k[n][0, ..., at] = bad
+        z = call_scan(on_gpu(k))
+        assert torch.equal(z[1], y[1]) and torch.equal(z[0, :, :at], y[0, :, :at])
+        assert n == "delta" or not z[0, :, at].isfinite().any()     # an infinite time step forgets all
+    dy = grads[0].clone()
+    dy[0, :, at] = bad
+    res = []
+    for up in (grads[0], dy):
+        c = {**on_gpu(i), **leaves_of(i)}
+        res.append(torch.autograd.grad(call_scan(c), [c[n] for n in ("x", "delta", "z", "B", "C")], up.cuda()))
+    for a, b in zip(*res):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[0, ..., at + 1:], b[0, ..., at + 1:])
+
+
 def test_scan_lengths_are_clamped():
     i, _ = scan_case("f32", 3, 2, 20, 3, lengths=[-5, 10 ** 12, 7])
     j = {**i, "lengths": torch.tensor([0, 20, 7])}
