@@ -15,7 +15,7 @@
 //
 // Measured at (8,2048,4096) bf16, 4 taps, SiLU: forward 62 us = 4.3 TB/s, backward 117 us = 3.4 TB/s (bytes alone:
 // 42 and 62 us at the measured copy rate); issue slots bound it, some 170 and 320 instructions for a warp's
-// 256 positions.  Rows of odd length, (3,768,16385) fp16: 40 us = 3.8 TB/s.
+// 256 positions.  Rows of odd length, (3,768,16385) fp16: 39 us = 3.9 TB/s.
 #pragma once
 
 #include "ssm_kernels.cuh"

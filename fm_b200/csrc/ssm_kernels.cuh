@@ -31,7 +31,7 @@
 // take 0.12 ms and the bytes 0.04 ms; backward 1.21 ms (0.12 ms, 0.07 ms).  What bounds them are the
 // latencies of the scan's dependent steps at 8 warps an SM (registers): per channel's tile of 64 positions
 // a warp of the forward issues some 280 instructions for the states and 100 for the positions, plus 550
-// per tile; backward 700, 240 and 800.
+// per tile; the backward about two and a half times as many.
 #pragma once
 
 #include "scan_kernels.cuh"
