@@ -184,15 +184,24 @@ __device__ __forceinline__ void stage_rows(unsigned char *to, int rows, int t0, 
     }
 }
 
-// The same where every granule is whole and aligned: lane `i` of `n` keeps one granule of every n / G-th row,
-// so its addresses advance by constants.  `from`: its granule of row i / G at t = 0.
+// The same where every granule lies inside the row (tile_inside): lane `i` of `n` keeps one granule of every
+// n / G-th row, so its addresses advance by constants, and the last one of a row that does not start on a
+// boundary also copies the one behind.  `from`: its granule of row i / G.
 template <typename S>
 constexpr int granules = kSsmTile * static_cast<int>(sizeof(S)) / 16;
-template <typename S>
+template <typename S, bool ALIGNED>
+__device__ __forceinline__ bool tile_inside(int t0, int len) {
+    return t0 + kSsmTile + (ALIGNED ? 0 : 16 / static_cast<int>(sizeof(S))) <= len;
+}
+template <typename S, bool ALIGNED>
 __device__ __forceinline__ void stage_whole(uint32_t dst, const S *from, int64_t stride, int rows, int i, int n) {
     const int step = n / granules<S>;
+    const bool behind = !ALIGNED && i % granules<S> == granules<S> - 1;
     for (int r = i / granules<S>; r < rows; r += step) {
-        copy16(dst, from, 16);
+        const unsigned char *at = reinterpret_cast<const unsigned char *>(from);
+        if (!ALIGNED) at -= reinterpret_cast<uintptr_t>(at) & 15;
+        copy16(dst, at, 16);
+        if (behind) copy16(dst + 16, at + 16, 16);
         dst += step * row_bytes<S>();
         from += step * stride;
     }
@@ -212,11 +221,36 @@ __device__ __forceinline__ int row_shift(const S *first) {
     return ALIGNED ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / sizeof(S));
 }
 
+// N words from the word `at` (< 4) of the 16-byte granules at `from` on.  Whole granules are read and the
+// words picked: loads of single words, 16 or 32 bytes apart from lane to lane, would meet the same few banks
+// (a training forward of (4,1024,4097) fp32: 442 us with them, 351 us so).
+template <int N>
+__device__ __forceinline__ void words_at(const unsigned char *from, int at, uint32_t (&w)[N]) {
+    constexpr int G = (N + 6) / 4;
+    const uint4 *q = reinterpret_cast<const uint4 *>(from);
+    uint32_t v[4 * G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+        const uint4 a = q[k];
+        v[4 * k] = a.x, v[4 * k + 1] = a.y, v[4 * k + 2] = a.z, v[4 * k + 3] = a.w;
+    }
+    const bool two = at & 2, one = at & 1;
+#pragma unroll
+    for (int k = 0; k < N + 1; ++k) v[k] = two ? v[k + 2] : v[k];
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] = one ? v[k + 1] : v[k];
+}
+
 // positions 4g ... 4g + 3 of a staged row
 template <typename S, bool ALIGNED>
 __device__ __forceinline__ void row_four(const unsigned char *row, int shift, int g, float (&f)[4]) {
     const S *p = reinterpret_cast<const S *>(row) + shift + 4 * g;
-    if constexpr (!ALIGNED) {
+    if constexpr (!ALIGNED && sizeof(S) == 4) {
+        uint32_t w[4];
+        words_at(row + 16 * g, shift, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    } else if constexpr (!ALIGNED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = Store<S>::to_float(p[i]);
     } else if constexpr (sizeof(S) == 4) {
@@ -238,24 +272,24 @@ __device__ __forceinline__ void row_eight(const unsigned char *row, int shift, i
             const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
             o[0] = pk(a.x, a.y), o[1] = pk(a.z, a.w), o[2] = pk(b.x, b.y), o[3] = pk(b.z, b.w);
         } else {
+            uint32_t w[8];
+            words_at(row + 32 * s, shift, w);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = pk(Store<S>::to_float(p[2 * k]), Store<S>::to_float(p[2 * k + 1]));
+            for (int k = 0; k < 4; ++k) o[k] = pk(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
         }
     } else {
         uint32_t w[4];
         if constexpr (ALIGNED) {
             const uint4 a = *reinterpret_cast<const uint4 *>(p);
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else {  // five words around the eight halfwords, shifted by one halfword where they start odd
-            const bool odd = shift & 1;
-            const uint32_t *q = reinterpret_cast<const uint32_t *>(p - (odd ? 1 : 0));
-            uint32_t v = q[0];
+        } else {  // five of the six words around the eight halfwords, shifted by one halfword where they start
+                  // odd; in 8-byte loads, which meet fewer banks twice than words do ((3,768,16386): 736 -> 692 us)
+            const uint2 *q = reinterpret_cast<const uint2 *>(row + 16 * s + (shift >> 2) * 8);
+            const uint2 a = q[0], b = q[1], c = q[2];
+            const bool one = shift & 2;
+            const uint32_t v[5] = {one ? a.y : a.x, one ? b.x : a.y, one ? b.y : b.x, one ? c.x : b.y, one ? c.y : c.x};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t next = (odd || k < 3) ? q[k + 1] : 0u;
-                w[k] = odd ? __funnelshift_r(v, next, 16) : v;
-                v = next;
-            }
+            for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], (shift & 1) * 16);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -535,16 +569,16 @@ ssm_forward_kernel(const SsmProblem<S> p, const float *__restrict__ carries, S *
     auto stage = [&](int tile, int nb, int step) {
         const int t0 = tile * kSsmTile;
         unsigned char *bc = ssm_smem + (step & 1) * (2 * kSsmNB * RB), *to = raw + (tile & 1) * (3 * p.cw * RB);
-        if (ALIGNED && t0 + kSsmTile <= len) {
+        if (ALIGNED && tile_inside<S, ALIGNED>(t0, len)) {  // unaligned rows too: 50 -> 54 us at (3,768,1001) fp16
             constexpr int n = kSsmFwdWarps * 32;
             if ((nb + 1) * kSsmNB <= p.N) {
-                stage_whole<S>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
-                stage_whole<S>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S, ALIGNED>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S, ALIGNED>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
             }
             if (nb == 0) {
-                stage_whole<S>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
-                stage_whole<S>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
-                if (p.z) stage_whole<S>(whole_dst<S>(to + 2 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
+                stage_whole<S, ALIGNED>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
+                stage_whole<S, ALIGNED>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
+                if (p.z) stage_whole<S, ALIGNED>(whole_dst<S>(to + 2 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
             }
         } else if (nb == 0) {
             stage_rows<S, ALIGNED>(to, w.nc, t0, len, lane, 32, any, [&](int c) { return xrow + c * p.xs[1]; });
@@ -552,7 +586,7 @@ ssm_forward_kernel(const SsmProblem<S> p, const float *__restrict__ carries, S *
             if (p.z)
                 stage_rows<S, ALIGNED>(to + 2 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return zrow + c * p.zs[1]; });
         }
-        if (!ALIGNED || t0 + kSsmTile > len || (nb + 1) * kSsmNB > p.N)
+        if (!ALIGNED || !tile_inside<S, ALIGNED>(t0, len) || (nb + 1) * kSsmNB > p.N)
             stage_rows<S, ALIGNED>(bc, 2 * kSsmNB, t0, len, threadIdx.x, kSsmFwdWarps * 32, any, [&](int r) -> const S * {
                 const int n = nb * kSsmNB + (r & (kSsmNB - 1));
                 return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
@@ -771,17 +805,17 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
                     for (int n = lane; n < p.N; n += 32) copy4(dst + (c * p.NP + n) * 4, ck + c * p.N + n);
             }
         }
-        if (ALIGNED && t0 + kSsmTile <= len) {
+        if (tile_inside<S, ALIGNED>(t0, len)) {
             constexpr int n = W * 32;
             if ((nb + 1) * kSsmNB <= p.N) {
-                stage_whole<S>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
-                stage_whole<S>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S, ALIGNED>(whole_dst<S>(bc, threadIdx.x), Bw + nb * kSsmNB * p.Bs[2] + t0, p.Bs[2], kSsmNB, threadIdx.x, n);
+                stage_whole<S, ALIGNED>(whole_dst<S>(bc + kSsmNB * RB, threadIdx.x), Cw + nb * kSsmNB * p.Cs[2] + t0, p.Cs[2], kSsmNB, threadIdx.x, n);
             }
             if (nb == 0) {
-                stage_whole<S>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
-                stage_whole<S>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
-                stage_whole<S>(whole_dst<S>(to + 2 * p.cw * RB, lane), gw + t0, T, w.nc, lane, 32);
-                if (GATED) stage_whole<S>(whole_dst<S>(to + 3 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
+                stage_whole<S, ALIGNED>(whole_dst<S>(to, lane), xw + t0, p.xs[1], w.nc, lane, 32);
+                stage_whole<S, ALIGNED>(whole_dst<S>(to + p.cw * RB, lane), dw + t0, p.ds[1], w.nc, lane, 32);
+                stage_whole<S, ALIGNED>(whole_dst<S>(to + 2 * p.cw * RB, lane), gw + t0, T, w.nc, lane, 32);
+                if (GATED) stage_whole<S, ALIGNED>(whole_dst<S>(to + 3 * p.cw * RB, lane), zw + t0, p.zs[1], w.nc, lane, 32);
             }
         } else if (nb == 0) {
             stage_rows<S, ALIGNED>(to, w.nc, t0, len, lane, 32, any, [&](int c) { return xrow + c * p.xs[1]; });
@@ -790,7 +824,7 @@ ssm_backward_kernel(const SsmProblem<S> p, const SsmGrads<S> o) {
             if (GATED)
                 stage_rows<S, ALIGNED>(to + 3 * p.cw * RB, w.nc, t0, len, lane, 32, any, [&](int c) { return zrow + c * p.zs[1]; });
         }
-        if (!ALIGNED || t0 + kSsmTile > len || (nb + 1) * kSsmNB > p.N)
+        if (!tile_inside<S, ALIGNED>(t0, len) || (nb + 1) * kSsmNB > p.N)
             stage_rows<S, ALIGNED>(bc, 2 * kSsmNB, t0, len, threadIdx.x, W * 32, any, [&](int r) -> const S * {
                 const int n = nb * kSsmNB + (r & (kSsmNB - 1));
                 return n >= p.N ? nullptr : r < kSsmNB ? Brow + n * p.Bs[2] : Crow + n * p.Cs[2];
